@@ -636,6 +636,109 @@ int rib_tp_reduce_add_rms(const rib_tp_prefill_exchange *ex, int M,
                           unsigned long long epoch, void *residual,
                           const void *norm_w, void *out, void *stream);
 
+/* ------------------------------------------------------------------------ *
+ * Paged KV cache (no counterpart in the reference, whose Cache is one
+ * contiguous buffer per request, agent-test/v2/engine.py:33-55).
+ *
+ * Unlike the entry points above, these take BF16 or FP16, any number of query
+ * heads per KV head, and strided tensors (strides in elements, multiples of
+ * 8; the last dimension is contiguous).  Row r of sequence s lies in page
+ * table[s][r / page_rows] at r % page_rows.  A table entry outside
+ * [0, num_pages) names no page; entries behind a sequence's rows are never
+ * read.  None of the calls keeps state or needs a cleared workspace, so calls
+ * on different streams, and captured graphs, are independent as long as each
+ * has buffers of its own.
+ *   pages   [num_pages][2][nkv][page_rows][head_dim], K then V
+ *   table   [seqs][width] int32, `table_stride` entries from row to row
+ * ------------------------------------------------------------------------ */
+#define RIB_DTYPE_BF16 0
+#define RIB_DTYPE_F16 1
+typedef struct rib_paged_cache {
+  void *pages;
+  const int32_t *table;
+  long long table_stride;
+  long long stride_page, stride_half, stride_head, stride_row;
+  int dtype, num_pages, nkv, page_rows, head_dim, seqs, width;
+} rib_paged_cache;
+
+/* Rotary positions: pair i of the first 2 * pairs dims of a head turns by
+ * pos * turns[i] turns (device FP64 table, 2 pi radians each), and is
+ * multiplied by `gain`.  pairs is a multiple of 8.  interleaved 0: pair i is
+ * dims (i, i + pairs); 1: dims (2 i, 2 i + 1). */
+typedef struct rib_rotary {
+  const double *turns;
+  int pairs, interleaved;
+  float gain;
+} rib_rotary;
+
+/* out[t][h] = x[t][h] rotated to position pos[t]: tokens x heads rows of
+ * `dim` (32..256, a multiple of 16) values.  out may be x itself. */
+int rib_rotary_apply(const rib_rotary *rot, const void *x, long long x_token,
+                     long long x_head, void *out, long long out_token,
+                     long long out_head, const int32_t *pos, int tokens,
+                     int heads, int dim, int dtype, void *stream);
+
+/* Append of `tokens` tokens: q_out = q rotated to pos[t]; k rotated and v as
+ * it is go to row row[t] of sequence seq[t] (seq NULL: sequence t).  With qw
+ * and kw [head_dim], q and k are first normalised per head: x w /
+ * sqrt(mean(x^2) + eps).  FP32 throughout, one rounding.  A negative row
+ * marks a padding token, for which nothing is written to the cache; a row or
+ * sequence the table names no page for writes nothing either and sets the
+ * device status word to RIB_ECAPACITY.  The (seq, row) pairs of a call must
+ * differ.  q_out may be q.  Serves agent-test/v2/engine.py:111-113 and
+ * :150-153 with pages in the place of Cache.update. */
+int rib_paged_append(const rib_paged_cache *cache, const rib_rotary *rot,
+                     const void *q, long long q_token, long long q_head,
+                     const void *k, long long k_token, long long k_head,
+                     const void *v, long long v_token, long long v_head,
+                     void *q_out, long long out_token, long long out_head,
+                     const int32_t *pos, const int32_t *row,
+                     const int32_t *seq, int tokens, int nq, const void *qw,
+                     const void *kw, float eps, void *stream);
+
+/* Attention of one new token per sequence over its lens[b] rows:
+ *   q [batch][nq][head_dim] (strides q_seq, q_head), out the same, contiguous;
+ *   nq a multiple of nkv; head_dim 64 or 128; page_rows a multiple of 16;
+ *   max_len >= every lens[b], at most width * page_rows.
+ * lens[b] == 0 gives a row of zeros.  With `scores` and `scores_out` (FP32
+ * [batch][nkv][>= max_len], rows contiguous; they may be the same buffer):
+ *   scores_out[b][h][n] = scores[b][h][n] + the softmax weight of row n
+ * summed over the query heads of KV head h, for n < lens[b]; entries behind
+ * stay as they are.  A length outside [0, max_len] is clamped and reported as
+ * RIB_ECAPACITY, a missing page reads as zeros and is reported as RIB_EINVAL
+ * (rib_take_device_status).
+ * workspace: rib_paged_decode_workspace_bytes(...) bytes, 16-byte aligned, of
+ * any content; calls that overlap on the device need one each. */
+size_t rib_paged_decode_workspace_bytes(int batch, int max_len, int nq,
+                                        int head_dim, int with_scores);
+int rib_paged_decode_attention(const rib_paged_cache *cache, const void *q,
+                               long long q_seq, long long q_head,
+                               const int32_t *lens, int batch, int nq,
+                               int max_len, float scale, void *out,
+                               const float *scores, long long scores_seq,
+                               long long scores_head, float *scores_out,
+                               long long out_seq, long long out_head,
+                               void *workspace, size_t workspace_bytes,
+                               void *stream);
+
+/* Eviction by score.  Each KV head of a sequence with more than `keep` rows
+ * keeps its first `sinks` rows, its last `recent` rows and, of those between,
+ * the keep - sinks - recent rows with the highest scores (equal scores: the
+ * lower row; NaN lowest); shorter sequences keep all.  The kept rows of K and
+ * V move, in order, to rows 0, 1, ... of new_table's pages (pages of the same
+ * tensor that the old table does not name), their scores to new_scores
+ * [batch][nkv][new_score_rows] (or NULL; zeros behind them; not overlapping
+ * scores).  rows [batch][nkv][keep] receives the old row numbers, -1 behind
+ * them, new_lens [batch] the new lengths.  head_dim 64 or 128. */
+int rib_paged_evict(const rib_paged_cache *cache, const int32_t *new_table,
+                    long long new_table_stride, int new_width,
+                    const int32_t *lens, int batch, int max_len,
+                    const float *scores, long long scores_seq,
+                    long long scores_head, int keep, int sinks, int recent,
+                    int32_t *rows, int32_t *new_lens, float *new_scores,
+                    long long new_seq, long long new_head,
+                    int new_score_rows, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

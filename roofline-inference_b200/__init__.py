@@ -18,6 +18,7 @@ from .kernels import (add_rms, argmax, embedding, gemv, qk_norm_rope, qk_norm_ro
                       swiglu)
 from .model import QWEN3_0_6B, DecodeGraph, Engine, Qwen3Config, Qwen3Weights, random_weights
 from .batch import BatchDecoder, SlotDecoder, generate_batch
+from .paged import Rotary, paged_append, paged_decode_attention, paged_evict, rotary
 from .pool import KVPool, PoolFull
 from .scheduler import Request, Scheduler
 
@@ -32,6 +33,7 @@ __all__ = [
     "Qwen3Config",
     "Qwen3Weights",
     "Request",
+    "Rotary",
     "Scheduler",
     "SlotDecoder",
     "add_rms",
@@ -41,8 +43,12 @@ __all__ = [
     "generate_batch",
     "qk_norm_rope_append_at",
     "qk_norm_rope_append_batched",
+    "paged_append",
+    "paged_decode_attention",
+    "paged_evict",
     "random_weights",
     "rms_norm",
+    "rotary",
     "swiglu",
     "attention",
     "decode_attention",

@@ -93,6 +93,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
 
 def _bind(L: ctypes.CDLL) -> None:
     vp, i, d, f, sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_double, ctypes.c_float, ctypes.c_size_t
+    ll = ctypes.c_longlong
     sig = {
         "rib_version": ([], i),
         "rib_status_string": ([i], ctypes.c_char_p),
@@ -127,6 +128,12 @@ def _bind(L: ctypes.CDLL) -> None:
         "rib_qk_norm_rope_append_batched": ([vp, vp, vp, vp, vp, vp, i, i, i, d, vp, vp], i),
         "rib_argmax_rows_f32": ([vp, i, i, vp, vp], i),
         "rib_decode_attention_qkv": ([vp, vp, vp, d, vp, vp, i, i, i, i, i, f, vp, vp, sz, vp], i),
+        "rib_rotary_apply": ([vp, vp, ll, ll, vp, ll, ll, vp, i, i, i, i, vp], i),
+        "rib_paged_append": ([vp, vp, vp, ll, ll, vp, ll, ll, vp, ll, ll, vp, ll, ll, vp, vp, vp, i, i, vp, vp, f,
+                              vp], i),
+        "rib_paged_decode_workspace_bytes": ([i, i, i, i, i], sz),
+        "rib_paged_decode_attention": ([vp, vp, ll, ll, vp, i, i, i, f, vp, vp, ll, ll, vp, ll, ll, vp, sz, vp], i),
+        "rib_paged_evict": ([vp, vp, ll, i, vp, i, i, vp, ll, ll, i, i, i, vp, vp, vp, ll, ll, i, vp], i),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)

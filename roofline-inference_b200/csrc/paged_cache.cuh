@@ -1,0 +1,43 @@
+// Paged KV cache: the device view that the paged kernels share.
+//
+// Pages are [num_pages][2][nkv][page_rows][D] (K, then V) of BF16 or FP16 values with a stride for
+// every dimension but the last; `table` [seqs][width] names the pages of each sequence in order, so
+// row r of sequence s lies in page table[s][r / page_rows] at r % page_rows.  A table entry outside
+// [0, num_pages) names no page: no kernel reads or writes through it.
+#pragma once
+
+#include "common.cuh"
+
+namespace rib {
+namespace paged {
+
+struct View {
+  uint16_t *pages;
+  const int32_t *table;
+  long long table_stride;                            // entries between two sequences
+  long long s_page, s_half, s_head, s_row;           // elements
+  int num_pages, nkv, page_rows, seqs, width;
+};
+
+// Two packed 16-bit values <-> FP32.
+struct BF16 {
+  static __device__ __forceinline__ float2 unpack(uint32_t w) { return make_float2(bf16lo(w), bf16hi(w)); }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
+};
+struct F16 {
+  static __device__ __forceinline__ float2 unpack(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_f16x2(lo, hi); }
+};
+
+// Page of row `r` of sequence `s`, or -1 where the table names none.
+__device__ __forceinline__ int page_of(const View &v, int s, int r) {
+  const int i = r / v.page_rows;
+  if (s < 0 || s >= v.seqs || r < 0 || i >= v.width) return -1;
+  const int page = __ldg(v.table + s * v.table_stride + i);
+  return page >= 0 && page < v.num_pages ? page : -1;
+}
+
+}  // namespace paged
+}  // namespace rib

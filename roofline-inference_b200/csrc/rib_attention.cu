@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <cstring>
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "decode_attention.cuh"
@@ -1416,3 +1417,5 @@ int rib_argmax_rows_f32(const float *x, int rows, int n, int32_t *out, void *str
 }
 
 }  // extern "C"
+
+#include "paged_api.cuh"

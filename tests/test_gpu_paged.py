@@ -1,0 +1,546 @@
+"""GPU: the paged-cache operators against their definitions in 64 bits (paged_ref.py).
+
+Tolerances: every result is rounded to its type once, so it may be off by half a step of that type
+(torch.finfo(t).eps / 2 relative) plus the FP32 arithmetic before it, whose bound is written where it
+is used.  Selections of rows and moved values must be exact."""
+from __future__ import annotations
+
+import importlib
+import math
+
+import pytest
+import torch
+
+from paged_ref import attend64, half_step, kept_rows, make_cache, rotate64, smallest_half
+
+pytestmark = pytest.mark.gpu
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module")
+def lib():
+    L = importlib.import_module("roofline-inference_b200._lib")
+    L.take_device_status()
+    return L
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def close(got, want, slack):
+    """|got - want| <= half a step of got's type + slack, element by element."""
+    d = (got.double() - want).abs()
+    lim = want.abs() * half_step(got.dtype) + smallest_half(got.dtype) + slack
+    bad = ~(d <= lim)
+    assert not bad.any(), (int(bad.sum()), float((d / lim)[bad].max()), bad.nonzero()[:3].tolist())
+
+
+# ------------------------------------------------------------------ rotary positions
+# FP32 arithmetic of a rotation, in units of 2^-24 of |a| + |b|: the norm's sum over 256 values in
+# chains of 16 and its shuffles (20 additions, halved by the root), root, quotient and two products (4),
+# the angle (half a turn rounded to FP32 is off by 2^-25 turns, 3.2 units of 2^-24 radians) and its sine
+# (2 ulp each), gain, two products and a sum (4): under 28 in all.
+ROT = 28 * 2.0 ** -24
+
+ROTATIONS = [
+    dict(head_dim=128), dict(head_dim=64, interleaved=True), dict(head_dim=128, rotary_dim=64),
+    dict(head_dim=64, rotary_dim=48, interleaved=True), dict(head_dim=96, rotary_dim=32, base=1e4),
+    dict(head_dim=256, rotary_dim=16), dict(head_dim=80, base=1e4), dict(head_dim=32, interleaved=True),
+    dict(head_dim=128, scaling="linear", factor=4.0), dict(head_dim=128, scaling="ntk", factor=8.0),
+    dict(head_dim=128, scaling="yarn", factor=4.0, original_length=4096, interleaved=True),
+    dict(head_dim=256, scaling="yarn", factor=32.0, original_length=32768),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("spec", ROTATIONS, ids=lambda s: "-".join(str(v) for v in s.values()))
+def test_rotary(rib, spec, dtype):
+    rot = rib.Rotary(**spec)
+    D = spec["head_dim"]
+    for tokens, heads in [(1, 1), (5, 3), (67, 33)]:
+        x = torch.randn((tokens, heads, D), generator=gen(tokens)).to(dtype).cuda()
+        pos = torch.randint(0, 1 << 21, (tokens,), generator=gen(1), dtype=torch.int32).cuda()
+        pos[0] = 0
+        want, size = rotate64(x, pos, rot.frequencies, rot.gain, rot.rotary_dim, rot.interleaved)
+        got = rib.rotary(x, pos, rot)
+        assert got.dtype == dtype and got.shape == x.shape
+        close(got, want, size * ROT)
+        assert torch.equal(got[..., rot.rotary_dim:], x[..., rot.rotary_dim:])  # the rest passes bit for bit
+        same = x.clone()
+        assert rib.rotary(same, pos, rot, out=same) is same and torch.equal(same, got)  # in place
+    assert rib.rotary(x[:0], pos[:0], rot).shape == (0, heads, D)
+
+
+def test_rotary_far_positions_and_strides(rib):
+    """The largest positions, and x as a transposed view into a wider buffer."""
+    rot = rib.Rotary(128)
+    wide = torch.randn((6, 9, 160), generator=gen(0)).to(BF16).cuda()
+    x = wide.transpose(0, 1)[:, 1:5, 16:144]
+    pos = i32([0, 1, 2 ** 17 + 1, 2 ** 24 + 1, 2 ** 31 - 1, -1, -70000, 12345, 2 ** 30])
+    before = wide.clone()
+    out = torch.zeros((4, 9, 128), dtype=BF16, device="cuda").transpose(0, 1)
+    got = rib.rotary(x, pos, rot, out=out)
+    want, size = rotate64(x, pos, rot.frequencies, rot.gain, 128, False)
+    close(got, want, size * ROT)
+    assert torch.equal(wide, before)
+
+
+# ------------------------------------------------------------------ append
+def check_append(rib, lib, *, T, nq, nkv, D, page_rows, dtype, norm, seqs, first, rot, seed=0, pages_view=None):
+    g = gen(seed)
+    share = -(-T // seqs)
+    seq = [t // share for t in range(T)]
+    row = [first + t % share for t in range(T)]
+    width = (first + share - 1) // page_rows + 2
+    total = seqs * width
+    pages = torch.randn((total + 2, 2, nkv, page_rows, D), generator=g).to(dtype).cuda()
+    if pages_view:
+        pages = pages_view(pages)
+    table = torch.randperm(total, generator=g).to(torch.int32).view(seqs, width).cuda()
+    qkv = torch.randn((T, (nq + 2 * nkv) * D), generator=g).to(dtype).cuda()
+    q, k, v = (s.view(T, -1, D) for s in qkv.split([nq * D, nkv * D, nkv * D], 1))
+    pos = torch.randint(0, 200000, (T,), generator=g, dtype=torch.int32).cuda()  # rows are not positions
+    qw = (1 + 0.2 * torch.randn(D, generator=g)).to(dtype).cuda() if norm else None
+    kw = (1 + 0.2 * torch.randn(D, generator=g)).to(dtype).cuda() if norm else None
+    want = pages.clone()
+    got_q = rib.paged_append(q, k, v, pos, i32(row), pages, table, rot, seq=i32(seq), qw=qw, kw=kw)
+    args = (pos, rot.frequencies, rot.gain, rot.rotary_dim, rot.interleaved)
+    q64, qs = rotate64(q, *args, w=qw)
+    k64, ks = rotate64(k, *args, w=kw)
+    close(got_q, q64, qs * ROT)
+    page = table[i32(seq).long(), i32(row).long() // page_rows].long()
+    slot = i32(row).long() % page_rows
+    close(pages[page, 0, :, slot], k64, ks * ROT)
+    assert torch.equal(pages[page, 1, :, slot], v)
+    want[page, :, :, slot] = pages[page, :, :, slot]
+    assert torch.equal(pages, want)  # nothing else was written
+    assert lib.take_device_status() == 0
+
+
+APPENDS = [
+    dict(T=1, nq=16, nkv=8, D=128, page_rows=16, dtype=BF16, norm=True, seqs=1, first=513),
+    dict(T=1, nq=1, nkv=1, D=64, page_rows=16, dtype=FP16, norm=False, seqs=1, first=0),
+    dict(T=5, nq=16, nkv=8, D=128, page_rows=64, dtype=BF16, norm=True, seqs=5, first=63),
+    dict(T=33, nq=6, nkv=2, D=64, page_rows=32, dtype=FP16, norm=True, seqs=2, first=30),
+    dict(T=300, nq=20, nkv=1, D=128, page_rows=16, dtype=BF16, norm=False, seqs=3, first=7),
+    dict(T=257, nq=4, nkv=4, D=256, page_rows=1, dtype=BF16, norm=True, seqs=1, first=0),
+    dict(T=9, nq=3, nkv=3, D=96, page_rows=5, dtype=FP16, norm=True, seqs=2, first=11),
+    dict(T=3001, nq=32, nkv=8, D=128, page_rows=256, dtype=FP16, norm=True, seqs=1, first=1),
+]
+
+
+@pytest.mark.parametrize("case", APPENDS, ids=lambda c: f"T{c['T']}-{c['nq']}x{c['nkv']}x{c['D']}-p{c['page_rows']}")
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append(rib, lib, case, interleaved):
+    D = case["D"]
+    check_append(rib, lib, rot=rib.Rotary(D, interleaved=interleaved), **case)
+    check_append(rib, lib, rot=rib.Rotary(D, rotary_dim=D // 2 // 16 * 16, interleaved=interleaved, scaling="yarn",
+                                          factor=4.0, original_length=8192), **case, seed=1)
+
+
+def test_append_into_one_layer_of_a_pool(rib, lib):
+    """Pages that are a slice of a larger tensor: every stride differs from the contiguous one."""
+    def view(pages):
+        pool = torch.randn((pages.shape[0], 3, 2, pages.shape[2], pages.shape[3], 2 * pages.shape[4]),
+                           generator=gen(9)).to(pages.dtype).cuda()
+        return pool[:, 1, ..., :pages.shape[4]]
+    check_append(rib, lib, rot=rib.Rotary(128), T=40, nq=4, nkv=2, D=128, page_rows=16, dtype=BF16, norm=True, seqs=4,
+                 first=10, pages_view=view)
+
+
+def test_append_padding_and_missing_pages(rib, lib):
+    """A negative row writes nothing; a row, sequence or page that is not there writes nothing and is reported."""
+    rot = rib.Rotary(64)
+    pages = torch.zeros((3, 2, 2, 16, 64), dtype=BF16, device="cuda")
+    table = i32([[0, 1], [2, -1]])
+    x = torch.randn((6, 2, 64), generator=gen(0)).to(BF16).cuda()
+
+    def call(seq, row):
+        pages.zero_()
+        q = rib.paged_append(x[:len(row)], x[:len(row)], x[:len(row)], i32([7] * len(row)), i32(row), pages, table,
+                             rot, seq=i32(seq))
+        assert torch.equal(q, rib.rotary(x[:len(row)], i32([7] * len(row)), rot))
+        return lib.take_device_status(), int((pages != 0).any(-1).any(1).any(1).sum())
+    assert call([0, 0, 1], [0, -1, -5]) == (0, 1)
+    assert call([0, 1], [17, 15]) == (0, 2)
+    for seq, row in [([0], [32]), ([1], [16]), ([2], [0]), ([-1], [3]), ([0], [2 ** 31 - 1])]:
+        assert call(seq, row) == (lib.RIB_ECAPACITY, 0)
+    table[0, 0] = 3  # outside the pool
+    assert call([0], [0]) == (lib.RIB_ECAPACITY, 0)
+
+
+# ------------------------------------------------------------------ attention
+def check_attention(rib, lib, lens, *, nq, nkv, D, page_rows, dtype, scores=False, seed=0, q_scale=1.0, fill=math.nan,
+                    max_len=None, width=None):
+    g = gen(seed)
+    B = len(lens)
+    pages, table = make_cache(lens, nkv, D, page_rows, dtype, g, fill=fill, width=width)
+    q = (torch.randn((B, nq, D), generator=g) * q_scale).to(dtype).cuda()
+    scale = D ** -0.5
+    want, weights, bound, rel = attend64(q, pages, table, lens, scale)
+    kw = {}
+    if scores:
+        room = table.shape[1] * page_rows
+        old = torch.rand((B, nkv, room + 3), generator=g).cuda()
+        new = torch.full_like(old, -7.0)
+        kw = dict(scores=old, scores_out=new)
+    got = rib.paged_decode_attention(q, pages, table, i32(lens), scale, max_len=max_len, **kw)
+    assert lib.take_device_status() == 0
+    close(got, want, bound)
+    if scores:
+        for b, n in enumerate(lens):
+            expect = old[b, :, :n].double() + weights[b]
+            assert ((new[b, :, :n].double() - expect).abs() <= expect * 2.0 ** -24 + weights[b] * rel[b]).all()
+            assert (new[b, :, n:] == -7.0).all()
+        again = old.clone()
+        out = rib.paged_decode_attention(q, pages, table, i32(lens), scale, max_len=max_len, scores=again)
+        assert torch.equal(out, got)
+        for b, n in enumerate(lens):
+            assert torch.equal(again[b, :, :n], new[b, :, :n]) and torch.equal(again[b, :, n:], old[b, :, n:])
+    return got
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("nq,nkv", [(1, 1), (16, 8), (10, 2), (8, 1), (18, 2), (20, 1)])
+def test_attention_heads_and_types(rib, lib, nq, nkv, D, dtype):
+    check_attention(rib, lib, [1, 15, 16, 17, 0, 33, 200], nq=nq, nkv=nkv, D=D, page_rows=16, dtype=dtype, scores=True)
+
+
+@pytest.mark.parametrize("page_rows", [16, 32, 48, 64, 256])
+def test_attention_pages_that_end_inside(rib, lib, page_rows):
+    check_attention(rib, lib, [page_rows - 1, page_rows, page_rows + 1, 3 * page_rows + 5, 1], nq=4, nkv=2, D=128,
+                    page_rows=page_rows, dtype=BF16, scores=page_rows == 48)
+
+
+@pytest.mark.parametrize("fill", [math.nan, math.inf, -math.inf, 3e38])
+def test_attention_ignores_what_lies_behind(rib, lib, fill):
+    """Rows behind the last one and pages no sequence names may hold anything."""
+    dtype = BF16
+    check_attention(rib, lib, [1, 9, 31, 130], nq=4, nkv=2, D=128, page_rows=32, dtype=dtype, fill=fill, scores=True)
+
+
+@pytest.mark.parametrize("lens", [[0], [0, 0, 0], [1], [4097], [0, 5000, 0, 3, 0], [16 * 8 + 1], [20000]])
+@pytest.mark.parametrize("scores", [False, True])
+def test_attention_lengths(rib, lib, lens, scores):
+    check_attention(rib, lib, lens, nq=4, nkv=2, D=128, page_rows=64, dtype=BF16, scores=scores)
+
+
+@pytest.mark.parametrize("B", [129, 700])
+def test_attention_many_sequences(rib, lib, B):
+    """More sequences than a CTA has threads, most of one tile, some empty."""
+    lens = [(b * 7919) % 40 if b % 5 else 0 for b in range(B)]
+    lens[B // 2] = 900
+    check_attention(rib, lib, lens, nq=2, nkv=1, D=64, page_rows=16, dtype=FP16, scores=True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_attention_sharp_and_large_scores(rib, lib, dtype):
+    """Scores in the hundreds: one row takes nearly all the weight, the running maximum moves."""
+    check_attention(rib, lib, [1000, 77], nq=4, nkv=2, D=128, page_rows=16, dtype=dtype, q_scale=40.0, scores=True)
+
+
+def test_attention_max_len_and_wide_table(rib, lib):
+    check_attention(rib, lib, [40, 100], nq=2, nkv=1, D=128, page_rows=16, dtype=BF16, max_len=100, width=50, scores=True)
+
+
+def test_attention_lengths_out_of_range_are_clamped(rib, lib):
+    g = gen(3)
+    pages, table = make_cache([64, 64], 1, 64, 16, BF16, g)
+    q = torch.randn((2, 2, 64), generator=g).to(BF16).cuda()
+    want = rib.paged_decode_attention(q, pages, table, i32([64, 0]), 0.125)
+    assert lib.take_device_status() == 0
+    got = rib.paged_decode_attention(q, pages, table, i32([65, -3]), 0.125)
+    assert lib.take_device_status() == lib.RIB_ECAPACITY
+    assert torch.equal(got, want)
+
+
+def test_attention_missing_page_is_reported(rib, lib):
+    g = gen(4)
+    pages, table = make_cache([64, 48], 1, 64, 16, BF16, g)
+    q = torch.randn((2, 2, 64), generator=g).to(BF16).cuda()
+    want = rib.paged_decode_attention(q, pages, table, i32([64, 48]), 0.125)
+    for bad in (-1, pages.shape[0], 2 ** 31 - 1):
+        t = table.clone()
+        t[1, 1] = bad
+        got = rib.paged_decode_attention(q, pages, t, i32([64, 48]), 0.125)
+        assert lib.take_device_status() == lib.RIB_EINVAL
+        assert torch.equal(got[0], want[0]) and torch.isfinite(got[1]).all()
+
+
+def test_attention_strided_inputs(rib, lib):
+    """q as a view of a projection, one layer of a pool, a table inside a wider one, a shared page."""
+    g = gen(5)
+    lens, nkv, D = [70, 33], 2, 128
+    pages, table = make_cache(lens, nkv, D, 16, BF16, g)
+    pool = torch.full((pages.shape[0], 3, 2, nkv, 16, 2 * D), math.nan, dtype=BF16, device="cuda")
+    pool[:, 1, ..., :D] = pages
+    table[1, 0] = table[0, 0]  # two sequences share their first page
+    wide = torch.full((2, 11), -1, dtype=torch.int32, device="cuda")
+    wide[:, 3:3 + table.shape[1]] = table
+    qkv = torch.randn((2, 8 * D), generator=g).to(BF16).cuda()
+    q = qkv[:, :4 * D].view(2, 4, D)
+    got = rib.paged_decode_attention(q, pool[:, 1, ..., :D], wide[:, 3:3 + table.shape[1]], i32(lens), 0.09)
+    want, _, bound, _ = attend64(q, pages, table, lens, 0.09)
+    close(got, want, bound)
+    assert lib.take_device_status() == 0
+
+
+def test_attention_beyond_32_bit_offsets(rib, lib):
+    """Pages whose first value lies past 2^31 values (4 GB) from the pool's start."""
+    g = gen(6)
+    pages, table = make_cache([100, 37], 2, 128, 64, BF16, g)
+    far = (1 << 31) // pages[0].numel() + 5
+    pool = torch.empty((far + pages.shape[0], *pages.shape[1:]), dtype=BF16, device="cuda")
+    pool[far:] = pages
+    q = torch.randn((2, 4, 128), generator=g).to(BF16).cuda()
+    want = rib.paged_decode_attention(q, pages, table, i32([100, 37]), 0.09)
+    assert torch.equal(rib.paged_decode_attention(q, pool, (table + (table >= 0) * far).int(), i32([100, 37]), 0.09), want)
+    # and the append and the eviction there
+    rot = rib.Rotary(128)
+    kv = torch.randn((2, 2, 128), generator=g).to(BF16).cuda()
+    rib.paged_append(q, kv, kv, i32([5, 6]), i32([99, 36]), pages, table, rot)
+    rib.paged_append(q, kv, kv, i32([5, 6]), i32([99, 36]), pool, (table + (table >= 0) * far).int(), rot)
+    assert torch.equal(pool[far:].nan_to_num(), pages.nan_to_num())
+    scores = torch.rand((2, 2, 128), generator=g).cuda()
+    free = [p for p in range(pages.shape[0]) if p not in table.tolist()[0] + table.tolist()[1]][:2]
+    new = i32([[free[0]], [free[1]]])
+    for t, pg, nt in ((table, pages, new), ((table + (table >= 0) * far).int(), pool, new + far)):
+        rows, n = rib.paged_evict(pg, t, i32([100, 37]), scores, 40, nt, sinks=2, recent=5)
+        assert n.tolist() == [40, 37]
+    assert torch.equal(pool[far:].nan_to_num(), pages.nan_to_num())
+    assert lib.take_device_status() == 0
+
+
+def test_attention_same_bits_every_time_and_on_every_stream(rib, lib):
+    """Results depend on nothing but the inputs: two streams at once, each with scratch of its own."""
+    g = gen(7)
+    lens = [3000, 1, 0, 700, 2049]
+    pages, table = make_cache(lens, 2, 128, 16, BF16, g)
+    q = torch.randn((5, 8, 128), generator=g).to(BF16).cuda()
+    want = rib.paged_decode_attention(q, pages, table, i32(lens), 0.09)
+    L = i32(lens)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = []
+    for _ in range(20):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(rib.paged_decode_attention(q, pages, table, L, 0.09))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+def test_capture_and_replay(rib, lib):
+    """A captured decode step (append, attention with scores) replays with what its buffers hold, and
+    two graphs captured one after the other run at the same time on two streams."""
+    g = gen(8)
+    nq, nkv, D, B = 4, 2, 128, 3
+    lens = [30, 500, 64]
+    rot = rib.Rotary(D)
+
+    def build(seed):
+        s = gen(seed)
+        pages, table = make_cache([n + 8 for n in lens], nkv, D, 16, BF16, s, fill=0.0)
+        st = dict(pages=pages, table=table, qkv=torch.zeros((B, (nq + 2 * nkv) * D), dtype=BF16, device="cuda"),
+                  pos=i32(lens), n=i32([x + 1 for x in lens]),
+                  scores=torch.zeros((B, nkv, table.shape[1] * 16), device="cuda"))
+        return st
+
+    def step(st):
+        q, k, v = (x.view(B, -1, D) for x in st["qkv"].split([nq * D, nkv * D, nkv * D], 1))
+        q = rib.paged_append(q, k, v, st["pos"], st["pos"], st["pages"], st["table"], rot)
+        out = rib.paged_decode_attention(q, st["pages"], st["table"], st["n"], 0.09, scores=st["scores"])
+        st["pos"].add_(1)
+        st["n"].add_(1)
+        return out
+
+    eager, captured = [build(1), build(2)], [build(1), build(2)]
+    inputs = [torch.randn((B, (nq + 2 * nkv) * D), generator=g).to(BF16).cuda() for _ in range(4)]
+    want = []
+    for i, st in enumerate(eager):
+        want.append([])
+        for x in inputs:
+            st["qkv"].copy_(x)
+            want[i].append(step(st).clone())
+    graphs, outs = [], []
+    for st in captured:
+        graph = torch.cuda.CUDAGraph()
+        keep = {k: st[k].clone() for k in ("pages", "pos", "n", "scores")}
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(st)
+        torch.cuda.current_stream().wait_stream(side)
+        for k, t in keep.items():
+            st[k].copy_(t)
+        with torch.cuda.graph(graph):
+            outs.append(step(st))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for x in inputs:
+        for i, st in enumerate(captured):
+            with torch.cuda.stream(streams[i]):
+                st["qkv"].copy_(x)
+                graphs[i].replay()
+                got[i].append(outs[i].clone())
+    torch.cuda.synchronize()
+    for i in range(2):
+        for a, b in zip(got[i], want[i]):
+            assert torch.equal(a, b)
+        assert torch.equal(captured[i]["scores"], eager[i]["scores"])
+        assert torch.equal(captured[i]["pages"], eager[i]["pages"])
+    assert lib.take_device_status() == 0
+
+
+# ------------------------------------------------------------------ eviction
+def check_evict(rib, lib, lens, *, nkv, D, page_rows, dtype, keep, sinks, recent, scores=None, seed=0, extra=0):
+    g = gen(seed)
+    B = len(lens)
+    new_need = [-(-min(n, keep) // page_rows) for n in lens]
+    pages, table = make_cache(lens, nkv, D, page_rows, dtype, g, spare=sum(new_need) + 1, fill=0.5)
+    free = sorted(set(range(pages.shape[0])) - set(table.flatten().tolist()))
+    width = max(1, -(-keep // page_rows))
+    new_table = torch.full((B, width), -1, dtype=torch.int32)
+    for b, m in enumerate(new_need):
+        for i in range(m):
+            new_table[b, i] = free.pop()
+    new_table = new_table.cuda()
+    room = table.shape[1] * page_rows
+    if scores is None:
+        scores = torch.rand((B, nkv, room), generator=g).cuda()
+    new_scores = torch.full((B, nkv, keep + extra), 9.0, device="cuda")
+    before, old_scores = pages.clone(), scores.clone()
+    rows, new_lens = rib.paged_evict(pages, table, i32(lens), scores, keep, new_table, sinks=sinks, recent=recent,
+                                     new_scores=new_scores)
+    assert lib.take_device_status() == 0
+    assert new_lens.tolist() == [min(n, keep) for n in lens]
+    want = before.clone()
+    host = scores.cpu()
+    for b, n in enumerate(lens):
+        for h in range(nkv):
+            kept = kept_rows(host[b, h], n, keep, sinks, recent)
+            assert rows[b, h].tolist() == kept + [-1] * (keep - len(kept)), (b, h)
+            src = torch.tensor(kept, dtype=torch.long, device="cuda")
+            dst = torch.arange(len(kept), device="cuda")
+            want[new_table[b, dst // page_rows].long(), :, h, dst % page_rows] = \
+                before[table[b, src // page_rows].long(), :, h, src % page_rows]
+            assert torch.equal(new_scores[b, h, :len(kept)].nan_to_num(-3), scores[b, h, src].nan_to_num(-3))
+            assert (new_scores[b, h, len(kept):] == 0).all()
+    assert torch.equal(pages, want)  # the old pages, and rows behind the kept ones, are as they were
+    assert torch.equal(scores.nan_to_num(-3), old_scores.nan_to_num(-3))
+    return rows
+
+
+@pytest.mark.parametrize("dtype,D,nkv,page_rows", [(BF16, 128, 2, 16), (FP16, 64, 3, 32), (BF16, 64, 1, 48)])
+@pytest.mark.parametrize("keep,sinks,recent", [(1, 0, 0), (1, 1, 0), (1, 0, 1), (40, 4, 8), (40, 20, 20), (100, 0, 99),
+                                               (64, 3, 0)])
+def test_evict(rib, lib, dtype, D, nkv, page_rows, keep, sinks, recent):
+    check_evict(rib, lib, [0, 1, keep, keep + 1, 300, 7], nkv=nkv, D=D, page_rows=page_rows, dtype=dtype, keep=keep,
+                sinks=sinks, recent=recent, extra=5)
+
+
+@pytest.mark.parametrize("n,keep", [(5000, 1234), (20001, 20000), (33000, 700)])
+def test_evict_long(rib, lib, n, keep):
+    check_evict(rib, lib, [n, n // 3], nkv=2, D=64, page_rows=64, dtype=BF16, keep=keep, sinks=4, recent=keep // 8)
+
+
+def test_evict_ties_infinities_and_nan(rib, lib):
+    """Equal scores go by the lower row, infinities rank as values, NaN lowest, -0 as 0."""
+    B, nkv, n = 6, 2, 160
+    s = torch.zeros((B, nkv, n))
+    s[1] = 1.0
+    s[2] = torch.arange(n) % 3
+    s[3] = torch.tensor([math.inf, -math.inf, 0.0, math.nan, -0.0, 5.0, -5.0, 1e-45]).repeat(n // 8)
+    s[4] = math.nan
+    s[5] = -torch.arange(n).float() * 1e30
+    s[:, 1] = s[:, 1].flip(-1)
+    for keep, sinks, recent in [(50, 3, 7), (81, 0, 0), (100, 1, 1), (159, 0, 0)]:
+        check_evict(rib, lib, [n] * B, nkv=nkv, D=64, page_rows=16, dtype=BF16, keep=keep, sinks=sinks, recent=recent,
+                    scores=s.cuda())
+
+
+def test_evict_reports_missing_pages(rib, lib):
+    g = gen(2)
+    pages, table = make_cache([64], 1, 64, 16, BF16, g, spare=2, fill=0.0)
+    free = sorted(set(range(pages.shape[0])) - set(table.flatten().tolist()))
+    scores = torch.rand((1, 1, 64), generator=g).cuda()
+    before = pages.clone()
+    rib.paged_evict(pages, table, i32([64]), scores, 32, i32([[free[0], -1]]))
+    assert lib.take_device_status() == lib.RIB_ECAPACITY
+    pages[free[0]] = before[free[0]]
+    assert torch.equal(pages, before)
+    rows, n = rib.paged_evict(pages, table, i32([65]), scores, 32, i32([free]))
+    assert lib.take_device_status() == lib.RIB_ECAPACITY and n.tolist() == [32]
+
+
+# ------------------------------------------------------------------ together
+@pytest.mark.parametrize("dtype,D,nq,nkv", [(BF16, 128, 4, 2), (FP16, 64, 6, 2)])
+def test_decode_with_eviction(rib, lib, dtype, D, nq, nkv):
+    """Append, attend and evict as a decode loop runs them, followed row by row in 64 bits: what a head
+    attends to after an eviction is exactly the rows that its scores kept."""
+    g = gen(11)
+    B, page_rows, keep, steps = 2, 16, 24, 60
+    rot = rib.Rotary(D)
+    pages = torch.zeros((40, 2, nkv, page_rows, D), dtype=dtype, device="cuda")
+    free = list(range(40))
+    width = 4
+    table = [[free.pop()] for _ in range(B)]
+    lens, pos = [0] * B, [0] * B
+    scores = torch.zeros((B, nkv, width * page_rows), device="cuda")
+    model = [[([], [], []) for _ in range(nkv)] for _ in range(B)]  # per head: keys, values, scores in FP64
+
+    def dev(t):
+        return i32([r + [-1] * (width - len(r)) for r in t])
+    for step in range(steps):
+        for b in range(B):
+            if lens[b] == len(table[b]) * page_rows:
+                table[b].append(free.pop())
+        q, k, v = (torch.randn((B, h, D), generator=g).to(dtype).cuda() for h in (nq, nkv, nkv))
+        qr = rib.paged_append(q, k, v, i32(pos), i32(lens), pages, dev(table), rot)
+        k64, _ = rotate64(k, i32(pos), rot.frequencies, 1.0, D, False)
+        lens = [n + 1 for n in lens]
+        pos = [p + 1 + (b == 1) for b, p in enumerate(pos)]
+        out = rib.paged_decode_attention(qr, pages, dev(table), i32(lens), D ** -0.5, scores=scores)
+        for b in range(B):
+            for h in range(nkv):
+                keys, vals, sc = model[b][h]
+                keys.append(k64[b, h].to(dtype).double())
+                vals.append(v[b, h].double())
+                sc.append(0.0)
+                K, V = torch.stack(keys), torch.stack(vals)
+                grp = slice(h * (nq // nkv), (h + 1) * (nq // nkv))
+                p = torch.softmax(qr[b, grp].double() @ K.T * D ** -0.5, -1)
+                # keys here are rounded from 64 bits, in the cache from 32: at most one step apart, so a
+                # score is off by at most 2 half steps of sum |q k|, and a weight by twice that
+                size = (qr[b, grp].double().abs() @ K.abs().T).amax().item() * D ** -0.5
+                e = 2 * 2 * half_step(dtype) * size + 2.0 ** -16
+                close(out[b, grp], p @ V, (p @ V.abs()) * e)
+                w = p.sum(0)
+                sc[:] = [a + x for a, x in zip(sc, w.tolist())]
+                got = scores[b, h, :lens[b]].double().cpu()
+                assert ((got - torch.tensor(sc, dtype=torch.float64)).abs() <= torch.tensor(sc) * (e + 1e-5)).all()
+        if step % 20 == 19 or max(lens) == width * page_rows:
+            new = [[free.pop() for _ in range(-(-min(n, keep) // page_rows))] for n in lens]
+            kept = torch.zeros_like(scores)
+            rows, n = rib.paged_evict(pages, dev(table), i32(lens), scores, keep, dev(new), sinks=2, recent=6,
+                                      new_scores=kept)
+            for b in range(B):
+                for h in range(nkv):
+                    at = [r for r in rows[b, h].tolist() if r >= 0]
+                    assert at == kept_rows(scores[b, h].cpu(), lens[b], keep, 2, 6)
+                    for lst in model[b][h][:2]:
+                        lst[:] = [lst[r] for r in at]
+                    model[b][h][2][:] = kept[b, h, :len(at)].tolist()
+            lens, scores = n.tolist(), kept
+            for b in range(B):
+                free.extend(table[b])
+            table = new
+    assert lib.take_device_status() == 0
