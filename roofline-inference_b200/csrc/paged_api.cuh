@@ -46,18 +46,25 @@ int rotary_ok(const rib_rotary *r, int dim) {
   return (reinterpret_cast<uintptr_t>(r->turns) & 7u) ? RIB_EALIGN : RIB_OK;
 }
 
+bool g_append_smem_done[2][5][kMaxDevices];
+
 template <class T, int LANES>
 int append_launch_lanes(rib::paged::AppendParams &p, cudaStream_t st) {
-  const long long items = p.nq + 2LL * p.nkv;
-  // One lane group per head while the GPU has lanes to spare; with more tokens a group takes several
-  // heads of its token and forms the token's cosines once for all of them.
-  const long long lanes = p.tokens * items * LANES, room = 1024LL * sm_count();
-  const long long heads = std::max(1LL, std::min(items, lanes / room));
-  p.groups = static_cast<int>((items + heads - 1) / heads);
-  const long long blocks = (p.tokens * static_cast<long long>(p.groups) * LANES + 255) / 256;
-  if (blocks > 0x7fffffffLL) return RIB_EINVAL;
-  return launch_pdl("append_kernel launch", rib::paged::append_kernel<T, LANES>, dim3(static_cast<unsigned>(blocks)),
-                    dim3(256), 0, st, p);
+  using namespace rib::paged;
+  // the lanes' rings, and (cos, sin) of 8 pairs of every lane
+  constexpr int smem = kAppendThreads * (kAppendStages * 32 + 8 * 8);
+  constexpr int which = LANES == 2 ? 0 : LANES == 4 ? 1 : LANES == 8 ? 2 : 3;
+  if (!set_smem_once(append_kernel<T, LANES>, smem, g_append_smem_done[std::is_same<T, F16>::value][which]))
+    return rib::host_fail(RIB_ECUDA, "cudaFuncSetAttribute(append smem)", smem);
+  // As many lane groups to a token as one wave holds, a head each at most: few tokens spread over the
+  // GPU, many keep their cosines for all their heads.
+  constexpr int in_cta = kAppendThreads / LANES;
+  const int items = p.nq + 2 * p.nkv, room = in_cta * kAppendCtas * sm_count();
+  p.groups = std::max(1, std::min(items, room / p.tokens));
+  p.inv_dim = 1.0f / static_cast<float>(p.dim);
+  const long long all = static_cast<long long>(p.tokens) * p.groups;
+  return launch_pdl("append_kernel launch", append_kernel<T, LANES>, dim3(ceil_div(all, in_cta)), dim3(kAppendThreads),
+                    smem, st, p);
 }
 
 template <class T>
@@ -68,9 +75,30 @@ int append_launch(rib::paged::AppendParams &p, cudaStream_t st) {
   return append_launch_lanes<T, 16>(p, st);
 }
 
+// launch_pdl with thread-block clusters of `ctas` CTAs along x.
+template <typename... KArgs, typename... Args>
+int launch_cluster(const char *what, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, int ctas,
+                   cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  return e == cudaSuccess ? RIB_OK : rib::host_fail_cuda(what, e);
+}
+
 // ------------------------------------------------------------------ paged decode
 struct PagedDecodeLayout {
-  size_t ml_off, rec_off, lse_off, logits_off, total;
+  size_t ml_off, rec_off, lse_off, span_off, logits_off, total;
   long long logit_row;
   int grid;
 };
@@ -85,9 +113,11 @@ PagedDecodeLayout paged_decode_layout(int batch, int max_len, int nq, int dim, b
   l.rec_off = off;
   off += round256(static_cast<size_t>(l.grid) * sizeof(JoinRecord));
   l.logit_row = (static_cast<long long>(max_len) + TK - 1) / TK * TK;
-  l.lse_off = l.logits_off = off;
+  l.lse_off = l.span_off = l.logits_off = off;
   if (scores) {
     off += round256(static_cast<size_t>(batch) * nq * sizeof(float));
+    l.span_off = off;  // at most one unit a query head
+    off += round256(static_cast<size_t>(batch) * nq * sizeof(int2));
     l.logits_off = off;
     off += round256(static_cast<size_t>(batch) * nq * l.logit_row * sizeof(float));
   }
@@ -114,6 +144,7 @@ bool paged_map(CUtensorMap *m, const rib_paged_cache *c) {
 }
 
 bool g_paged_smem_done[2][2][2][kMaxDevices];
+bool g_select_smem_done[kMaxDevices];
 
 template <class T, int D, bool kLogits>
 int paged_decode_launch(const rib::paged::DecodeParams &p, int grid, cudaStream_t st) {
@@ -124,7 +155,11 @@ int paged_decode_launch(const rib::paged::DecodeParams &p, int grid, cudaStream_
     return rib::host_fail(RIB_ECUDA, "cudaFuncSetAttribute(paged decode smem)", smem);
   const int s = launch_pdl("paged_decode_kernel launch", kernel, dim3(grid), dim3(NT), smem, st, p);
   if (s != RIB_OK) return s;
-  return launch_pdl("join_kernel launch", join_kernel<T, D>, dim3(grid), dim3(256), 0, st, p);
+  const int row_blocks = kLogits ? ceil_div(p.max_len, kWeightRows) : 0;
+  const long long blocks = grid + static_cast<long long>(row_blocks) * p.cache.nkv * p.batch;
+  if (blocks > 0x7fffffffLL) return RIB_EINVAL;
+  return launch_pdl("join_kernel launch", join_kernel<T, D>, dim3(static_cast<unsigned>(blocks)), dim3(kJoinThreads), 0,
+                    st, p, grid, row_blocks);
 }
 
 template <class T>
@@ -236,7 +271,8 @@ int rib_paged_decode_attention(const rib_paged_cache *cache, const void *q, long
       max_len > static_cast<long long>(cache->width) * cache->page_rows || !(scale > 0.f) || !(scale < INFINITY) ||
       (dim != 64 && dim != 128) || cache->page_rows % TK || !scores != !scores_out)
     return RIB_EINVAL;
-  if (scores && (batch > 65535 || cache->nkv > 65535)) return RIB_EINVAL;
+  if (scores && static_cast<long long>(batch) * cache->nkv * ceil_div(max_len, kWeightRows) > 0x7fff0000LL)
+    return RIB_EINVAL;
   const PagedDecodeLayout l = paged_decode_layout(batch, max_len, nq, dim, scores != nullptr);
   if (!workspace || workspace_bytes < l.total) return RIB_EINVAL;
   if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || !aligned4(lens) || !aligned4(scores) ||
@@ -262,28 +298,18 @@ int rib_paged_decode_attention(const rib_paged_cache *cache, const void *q, long
   p.logit_row = l.logit_row;
   if (scores) {
     p.lse = reinterpret_cast<float *>(ws + l.lse_off);
+    p.span = reinterpret_cast<int2 *>(ws + l.span_off);
     p.logits = reinterpret_cast<float *>(ws + l.logits_off);
+    p.scores = scores;
+    p.scores_out = scores_out;
+    p.in_seq = scores_seq;
+    p.in_head = scores_head;
+    p.out_seq = out_seq;
+    p.out_head = out_head;
   }
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int s = cache->dtype == RIB_DTYPE_F16 ? paged_decode_launch<F16>(p, dim, l.grid, st)
-                                              : paged_decode_launch<BF16>(p, dim, l.grid, st);
-  if (s != RIB_OK || !scores) return s;
-  WeightParams w;
-  w.logits = p.logits;
-  w.lse = p.lse;
-  w.scores = scores;
-  w.scores_out = scores_out;
-  w.lens = lens;
-  w.logit_row = l.logit_row;
-  w.in_seq = scores_seq;
-  w.in_head = scores_head;
-  w.out_seq = out_seq;
-  w.out_head = out_head;
-  w.nq = nq;
-  w.group = p.group;
-  w.max_len = max_len;
-  return launch_pdl("row_weight_kernel launch", row_weight_kernel,
-                    dim3(ceil_div(max_len, 1024), cache->nkv, batch), dim3(256), 0, st, w);
+  return cache->dtype == RIB_DTYPE_F16 ? paged_decode_launch<F16>(p, dim, l.grid, st)
+                                       : paged_decode_launch<BF16>(p, dim, l.grid, st);
 }
 
 int rib_paged_evict(const rib_paged_cache *cache, const int32_t *new_table, long long new_table_stride, int new_width,
@@ -326,14 +352,22 @@ int rib_paged_evict(const rib_paged_cache *cache, const int32_t *new_table, long
   s.recent = recent;
   s.max_len = max_len;
   s.new_width = new_score_rows;
-  const int e = launch_pdl("select_rows_kernel launch", select_rows_kernel, dim3(cache->nkv, batch), dim3(kSelThreads),
-                           0, st, s);
+  // CTAs of a cluster: more while they fit one wave and each still has 4096 rows
+  int ctas = 1;
+  while (ctas < 8 && 2LL * ctas * batch * cache->nkv <= 2 * sm_count() && max_len >= 8192 * ctas) ctas *= 2;
+  const int part = ceil_div(max_len, ctas * kSelThreads) * kSelThreads;
+  const bool fits = part <= kSelMostRows;
+  const auto select = fits ? select_rows_kernel<true> : select_rows_kernel<false>;
+  constexpr int most = kSelMostRows * static_cast<int>(sizeof(float));
+  if (!set_smem_once(select_rows_kernel<true>, most, g_select_smem_done))
+    return rib::host_fail(RIB_ECUDA, "cudaFuncSetAttribute(select smem)", most);
+  const int e = launch_cluster("select_rows_kernel launch", select, dim3(cache->nkv * ctas, batch), dim3(kSelThreads),
+                               fits ? part * sizeof(float) : 0, ctas, st, s);
   if (e != RIB_OK) return e;
   m.rows = rows;
   m.keep = keep;
-  m.dim = cache->head_dim;
-  return launch_pdl("move_rows_kernel launch", move_rows_kernel, dim3(ceil_div(keep, 256), cache->nkv, batch),
-                    dim3(256), 0, st, m);
+  return launch_pdl("move_rows_kernel launch", cache->head_dim == 128 ? move_rows_kernel<128> : move_rows_kernel<64>,
+                    dim3(ceil_div(keep, kMoveThreads / 32 * kMoveRows), cache->nkv, batch), dim3(kMoveThreads), 0, st, m);
 }
 
 }  // extern "C"

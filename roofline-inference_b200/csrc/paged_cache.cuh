@@ -23,12 +23,14 @@ struct View {
 struct BF16 {
   static __device__ __forceinline__ float2 unpack(uint32_t w) { return make_float2(bf16lo(w), bf16hi(w)); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
+  static __device__ __forceinline__ float one(uint16_t v) { return bf16lo(v); }
 };
 struct F16 {
   static __device__ __forceinline__ float2 unpack(uint32_t w) {
     return __half22float2(*reinterpret_cast<const __half2 *>(&w));
   }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_f16x2(lo, hi); }
+  static __device__ __forceinline__ float one(uint16_t v) { return __half2float(__ushort_as_half(v)); }
 };
 
 // Page of row `r` of sequence `s`, or -1 where the table names none.

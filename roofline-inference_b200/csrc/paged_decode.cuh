@@ -50,10 +50,12 @@ struct DecodeSmem {
   alignas(16) float o[NW - 1][HU][D];
   float m[NW][HU], l[NW][HU];
   uint64_t full[NW][DecodeCfg<D>::ST];
-  long long start[2];                             // first sequence of the run, tiles before it
+  long long sum[NW];                              // tiles of each warp's sequences
+  long long start_tiles;                          // tiles before the run's first sequence
+  int start_seq, start_rows;                      // that sequence and its rows
 };
 
-// A unit that spans CTAs: its first CTA is the record's own, `last` its last one.
+// The unit that begins in a CTA's run and ends in CTA `last`'s (-1: there is none).
 struct JoinRecord {
   int b, hu, last;
 };
@@ -72,7 +74,11 @@ struct DecodeParams {
   float *part_ml;               // [grid][2][HU][2]
   JoinRecord *rec;              // [grid]
   float *logits;                // [B][nq][logit_row] scores in log2 units, or null
-  float *lse;                   // [B][nq] log2 of the sum, with logits
+  float *lse;                   // [B][nq] log2 of the sum of units of one CTA, with logits
+  int2 *span;                   // [B][units] first and last CTA of a unit that spans several, or -1
+  const float *scores;          // row weights: scores_out = scores + weight, strides below
+  float *scores_out;
+  long long in_seq, in_head, out_seq, out_head;
   long long logit_row;          // max_len rounded up to whole tiles
 };
 
@@ -146,7 +152,6 @@ __global__ void __launch_bounds__(NT, kCtasPerSm) paged_decode_kernel(const __gr
   extern __shared__ uint8_t smem_raw[];
   DecodeSmem<D> &sm = *reinterpret_cast<DecodeSmem<D> *>(
       smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
-  __shared__ long long warp_sum[NW];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int units = p.cache.nkv * p.units_per_kv;
 
@@ -162,9 +167,12 @@ __global__ void __launch_bounds__(NT, kCtasPerSm) paged_decode_kernel(const __gr
   const int per = (p.batch + NT - 1) / NT;
   const int b_lo = min(tid * per, p.batch), b_hi = min(b_lo + per, p.batch);
   long long mine = 0;
+  int first_rows = 0;
   for (int b = b_lo; b < b_hi; ++b) {
-    mine += seq_tiles(p, b);
-    if (blockIdx.x == 0 && (p.lens[b] < 0 || p.lens[b] > p.max_len)) atomicExch(&g_device_status, RIB_ECAPACITY);
+    const int n = seq_rows(p, b);
+    if (b == b_lo) first_rows = n;
+    mine += (n + TK - 1) / TK;
+    if (blockIdx.x == 0 && n != p.lens[b]) atomicExch(&g_device_status, RIB_ECAPACITY);
   }
   long long inc = mine;
 #pragma unroll
@@ -172,91 +180,95 @@ __global__ void __launch_bounds__(NT, kCtasPerSm) paged_decode_kernel(const __gr
     const long long up = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += up;
   }
-  if (lane == 31) warp_sum[warp] = inc;
+  if (lane == 31) sm.sum[warp] = inc;
   __syncthreads();
   long long before = inc - mine, all = 0;
+#pragma unroll
   for (int w = 0; w < NW; ++w) {
-    if (w < warp) before += warp_sum[w];
-    all += warp_sum[w];
+    if (w < warp) before += sm.sum[w];
+    all += sm.sum[w];
   }
   all *= units;
-  // few tiles: fewer CTAs, each with kMinTiles at least
-  const long long grid = min(static_cast<long long>(gridDim.x), (all + kMinTiles - 1) / kMinTiles);
+  // Few tiles: fewer CTAs, each with kMinTiles at least.  CTA i takes `quot` tiles, the first `rest` one more.
   const int cta = blockIdx.x;
-  if (cta < grid) {
-    const long long s0 = cta * all / grid;
-    if (mine > 0 && before * units <= s0 && s0 < (before + mine) * units) {
-      long long at = before;
-      int b = b_lo;
-      for (;; ++b) {
-        const int tb = seq_tiles(p, b);
-        if (s0 < (at + tb) * units) break;
-        at += tb;
-      }
-      sm.start[0] = b;
-      sm.start[1] = at * units;
+  const int grid = all < static_cast<long long>(gridDim.x) * kMinTiles
+                       ? (static_cast<int>(all) + kMinTiles - 1) / kMinTiles : gridDim.x;
+  const long long quot = !grid ? 0 : all >> 31 ? all / grid : static_cast<int>(all) / grid;
+  const int rest = static_cast<int>(all - quot * grid);
+  const long long s0 = cta * quot + min(cta, rest);
+  const int run = cta < grid ? static_cast<int>(quot + (cta < rest)) : 0;
+  if (run && before * units <= s0 && s0 < (before + mine) * units) {
+    int b = b_lo, n = first_rows;
+    while (s0 >= (before + (n + TK - 1) / TK) * units) {
+      before += (n + TK - 1) / TK;
+      n = seq_rows(p, ++b);
     }
+    sm.start_seq = b;
+    sm.start_rows = n;
+    sm.start_tiles = before * units;
   }
   __syncthreads();
-  // sequences without rows get zeros (and no tiles): spread over the grid
+  if (!run && tid == 0) p.rec[cta].last = -1;
+  // sequences without rows have no tiles, and get zeros
   for (int b = cta; b < p.batch; b += gridDim.x) {
     if (seq_rows(p, b) > 0) continue;
     for (int i = tid; i < p.nq * (D / 2); i += NT)
       reinterpret_cast<uint32_t *>(p.out + static_cast<size_t>(b) * p.nq * D)[i] = 0;
   }
-  if (cta >= grid) {
-    if (tid == 0 && cta < gridDim.x) p.rec[cta].last = -1;
-    return;
-  }
-  const long long s0 = cta * all / grid, s1 = (cta + 1) * all / grid;
+  if (!run) return;
   Place c;
-  c.b = static_cast<int>(sm.start[0]);
-  c.n = seq_rows(p, c.b);
+  c.b = sm.start_seq;
+  c.n = sm.start_rows;
   c.tiles = (c.n + TK - 1) / TK;
   {
-    const long long in_seq = s0 - sm.start[1];
-    c.hu = static_cast<int>(in_seq / c.tiles);
-    c.tile = static_cast<int>(in_seq % c.tiles);
+    const long long in_seq = s0 - sm.start_tiles;
+    c.hu = in_seq >> 31 ? static_cast<int>(in_seq / c.tiles) : static_cast<int>(in_seq) / c.tiles;
+    c.tile = static_cast<int>(in_seq - static_cast<long long>(c.hu) * c.tiles);
   }
-  const int run = static_cast<int>(s1 - s0);
 
-  // ---- producer side of the warp: lane 0 copies tile after tile of this warp
-  Place pc = c;
-  int issued = 0, pf = warp;  // tiles issued; run index of the next one
-  int page_next = -1;
-  // moves pc on by `by` tiles, then reads the next tile's page number
-  auto seek = [&](int by) {
-    if (pf >= run) return;
-    pc.tile += by;
-    while (pc.tile >= pc.tiles) {
-      const int over = pc.tile - pc.tiles;
-      if (!next_unit(p, pc, units)) return;  // cannot happen while pf < run
-      pc.tile = over;
+  // ---- producer side of the warp: tile i of the warp is the run's tile warp + i * NW
+  const int count = run > warp ? (run - warp + NW - 1) / NW : 0;
+  // moves `by` tiles along the run
+  auto seek = [&](Place &pl, int by) {
+    pl.tile += by;
+    while (pl.tile >= pl.tiles) {
+      const int over = pl.tile - pl.tiles;
+      if (!next_unit(p, pl, units)) return;  // never within the run
+      pl.tile = over;
     }
-    const int i = pc.tile * TK / p.cache.page_rows;
-    page_next = i < p.cache.width ? __ldg(p.cache.table + pc.b * p.cache.table_stride + i) : -1;
   };
-  auto issue = [&]() {
-    if (pf >= run) return;
-    const int slot = issued % ST;
-    if (page_next < 0 || page_next >= p.cache.num_pages) {
+  auto page_at = [&](const Place &pl) {
+    return __ldg(p.cache.table + pl.b * p.cache.table_stride + pl.tile * TK / p.cache.page_rows);
+  };
+  auto copy = [&](const Place &pl, int page, int slot) {
+    if (page < 0 || page >= p.cache.num_pages) {
       atomicExch(&g_device_status, RIB_EINVAL);
-      page_next = p.cache.num_pages;  // outside the map: the box reads as zeros
+      page = p.cache.num_pages;  // outside the map: the box reads as zeros
     }
     mbar_arrive_expect_tx(&sm.full[warp][slot], Cfg::STAGE);
 #pragma unroll
     for (int hf = 0; hf < D / 64; ++hf)
-      tma_load_5d(sm.ring[warp][slot] + hf * Cfg::HALF, &p.map, 64 * hf, pc.tile * TK % p.cache.page_rows,
-                  pc.hu / p.units_per_kv, 0, page_next, &sm.full[warp][slot]);
-    ++issued;
-    pf += NW;
-    seek(NW);
+      tma_load_5d(sm.ring[warp][slot] + hf * Cfg::HALF, &p.map, 64 * hf, pl.tile * TK % p.cache.page_rows,
+                  pl.hu / p.units_per_kv, 0, page, &sm.full[warp][slot]);
   };
-  if (lane == 0) {
-    seek(warp);
-#pragma unroll 1
-    for (int i = 0; i < ST; ++i) issue();
+  if (lane < min(ST, count)) {  // the first tiles, a lane each
+    Place pl = c;
+    seek(pl, warp + lane * NW);
+    copy(pl, page_at(pl), lane);
   }
+  Place pc = c;  // lane 0: the next tile to copy, its page asked for, and looked at only then
+  int issued = min(ST, count), page_next = 0;
+  if (lane == 0 && issued < count) {
+    seek(pc, warp + issued * NW);
+    page_next = page_at(pc);
+  }
+  auto issue = [&]() {
+    copy(pc, page_next, issued % ST);
+    if (++issued < count) {
+      seek(pc, NW);
+      page_next = page_at(pc);
+    }
+  };
   __syncwarp();
 
   const int g = lane >> 2, t4 = lane & 3;
@@ -361,7 +373,7 @@ __global__ void __launch_bounds__(NT, kCtasPerSm) paged_decode_kernel(const __gr
         mma16816<T>(o[ch + 1], a0, a1, a2, a3, vb[2], vb[3]);
       }
       __syncwarp();  // every lane has read the slot
-      if (lane == 0) issue();
+      if (lane == 0 && issued < count) issue();
     }
 
     // ---- the warps' results of this unit: scaled to a common maximum, summed in warp order
@@ -415,75 +427,147 @@ __global__ void __launch_bounds__(NT, kCtasPerSm) paged_decode_kernel(const __gr
           p.lse[static_cast<size_t>(c.b) * p.nq + h0 + g] = L == 0.f ? INFINITY : M + log2f(L);
         }
       }
-      if (lane == 0 && f + seg == run) {  // the run's last unit: does it begin here and end elsewhere?
-        JoinRecord r = {c.b, c.hu, -1};
-        if (c.tile == 0 && seg < c.tiles) {
-          const long long end = s0 + f + c.tiles;  // one behind the unit's last tile
-          r.last = static_cast<int>((end * grid - 1) / all);
+      if (lane == 0) {
+        int last = -1;  // the CTA in which a unit that begins here and does not end here ends
+        if (c.tile == 0 && !whole) {
+          const long long x = s0 + f + c.tiles - 1, big = rest * (quot + 1);  // its last tile
+          last = static_cast<int>(x < big ? x / (quot + 1) : rest + (x - big) / quot);
         }
-        p.rec[cta] = r;
+        if (f + seg == run) p.rec[cta] = {c.b, c.hu, last};
+        if (kLogits && c.tile == 0) p.span[static_cast<size_t>(c.b) * units + c.hu] = make_int2(cta, last);
       }
     }
     f += seg;
     if (f < run) next_unit(p, c, units);
   }
   if (dead) {  // copies still under way must land before the CTA's shared memory is given up
-    const int n_issued = __shfl_sync(0xffffffffu, issued, 0);
-    for (int i = max(0, n_issued - ST); i < n_issued; ++i) mbar_wait(&sm.full[warp][i % ST], (i / ST) & 1);
+    const int sent = __shfl_sync(0xffffffffu, issued, 0);
+    for (int i = max(0, sent - ST); i < sent; ++i) mbar_wait(&sm.full[warp][i % ST], (i / ST) & 1);
   }
 }
 
-// Joins the partials of a unit that spans CTAs, in run order: one CTA per CTA of the split launch.
+constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * 32;
+constexpr int kWeightRows = 1024;  // rows of a weight block
+
+// Place of CTA c's partial of a unit that begins in CTA `first`: that one's second, the others' first.
+__device__ __forceinline__ size_t part_slot(int c, int first) { return static_cast<size_t>(c) * 2 + (c == first); }
+
+// Maximum and sum of head g of a unit over its partials, by a whole warp (in every lane, in CTA order
+// within a lane and by a fixed tree over the lanes).
+__device__ __forceinline__ float2 joined_ml(const DecodeParams &p, int first, int last, int g, int lane) {
+  float M = -INFINITY, L = 0.f;
+  for (int c = first + lane; c <= last; c += 32) {
+    const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + (part_slot(c, first) * HU + g) * 2);
+    const float mn = fmaxf(M, ml.x), mz = mn == -INFINITY ? 0.f : mn;
+    L = L * fast_exp2(M - mz) + ml.y * fast_exp2(ml.x - mz);
+    M = mn;
+  }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, M, o), l2 = __shfl_xor_sync(0xffffffffu, L, o);
+    const float mn = fmaxf(M, m2), mz = mn == -INFINITY ? 0.f : mn;
+    L = L * fast_exp2(M - mz) + l2 * fast_exp2(m2 - mz);
+    M = mn;
+  }
+  return make_float2(M, L);
+}
+
+// Blocks below `grid`: join the unit that begins in that CTA's run and ends in another's.  The warps
+// take (head, slice of the partials), so all partials are under way at once; the slices are summed in
+// order.  With scores, the blocks behind add the row weights of kWeightRows rows of one KV head each.
 template <class T, int D>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ DecodeParams p) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ DecodeParams p, int grid,
+                                                            int row_blocks) {
+  __shared__ float4 acc[kJoinWarps][D / 4];
+  __shared__ float head_sum[kJoinWarps];
   pdl_launch_dependents();
   pdl_wait();
-  const JoinRecord r = p.rec[blockIdx.x];
-  if (r.last < 0) return;
-  const int first = blockIdx.x, kvh = r.hu / p.units_per_kv, g0 = (r.hu % p.units_per_kv) * HU;
-  const int heads = min(HU, p.group - g0), h0 = kvh * p.group + g0;
-  for (int i = threadIdx.x; i < heads * (D / 2); i += blockDim.x) {
-    const int g = i / (D / 2), d = i % (D / 2) * 2;
-    // the first CTA's second partial, then the first partial of those behind it
-    auto slot = [&](int c) { return static_cast<size_t>(c) * 2 + (c == first ? 1 : 0); };
-    float M = -INFINITY;
-    for (int c = first; c <= r.last; ++c) M = fmaxf(M, p.part_ml[(slot(c) * HU + g) * 2]);
-    float L = 0.f;
-    float2 o = make_float2(0.f, 0.f);
-    for (int c = first; c <= r.last; ++c) {
-      const float2 ml = *reinterpret_cast<const float2 *>(p.part_ml + (slot(c) * HU + g) * 2);
-      const float2 v = *reinterpret_cast<const float2 *>(p.part_o + (slot(c) * HU + g) * D + d);
-      const float al = M == -INFINITY ? 0.f : fast_exp2(ml.x - M);
-      L = fmaf(ml.y, al, L);
-      o.x = fmaf(v.x, al, o.x);
-      o.y = fmaf(v.y, al, o.y);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (static_cast<int>(blockIdx.x) < grid) {
+    const JoinRecord r = p.rec[blockIdx.x];
+    if (r.last < 0) return;
+    const int first = blockIdx.x, kvh = r.hu / p.units_per_kv, g0 = (r.hu % p.units_per_kv) * HU;
+    const int heads = min(HU, p.group - g0), h0 = kvh * p.group + g0;
+    const int slices = kJoinWarps / heads, g = warp / slices, slice = warp % slices;
+    constexpr int V = D / 4, R = 32 / V;  // lanes of a row, rows of a load
+    const int v = lane % V, sub = lane / V;
+    if (g < heads) {
+      const float2 ml = joined_ml(p, first, r.last, g, lane);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int c = first + slice * R + sub; c <= r.last; c += slices * R) {
+        const size_t s = part_slot(c, first) * HU + g;
+        const float4 u = *reinterpret_cast<const float4 *>(p.part_o + s * D + 4 * v);
+        const float al = ml.x == -INFINITY ? 0.f : fast_exp2(p.part_ml[2 * s] - ml.x);
+        o.x = fmaf(u.x, al, o.x);
+        o.y = fmaf(u.y, al, o.y);
+        o.z = fmaf(u.z, al, o.z);
+        o.w = fmaf(u.w, al, o.w);
+      }
+      if (R == 2) {
+        o.x += __shfl_xor_sync(0xffffffffu, o.x, 16);
+        o.y += __shfl_xor_sync(0xffffffffu, o.y, 16);
+        o.z += __shfl_xor_sync(0xffffffffu, o.z, 16);
+        o.w += __shfl_xor_sync(0xffffffffu, o.w, 16);
+      }
+      if (sub == 0) acc[warp][v] = o;
+      if (lane == 0) head_sum[warp] = ml.y;
     }
-    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-    const size_t head = static_cast<size_t>(r.b) * p.nq + h0 + g;
-    *reinterpret_cast<uint32_t *>(p.out + head * D + d) = T::pack(o.x * inv, o.y * inv);
-    if (p.lse && d == 0) p.lse[head] = L == 0.f ? INFINITY : M + log2f(L);
+    __syncthreads();
+    for (int i = tid; i < heads * V; i += kJoinThreads) {
+      const int hg = i / V, d = i % V;
+      float4 o = acc[hg * slices][d];
+      for (int k = 1; k < slices; ++k) {
+        const float4 u = acc[hg * slices + k][d];
+        o = make_float4(o.x + u.x, o.y + u.y, o.z + u.z, o.w + u.w);
+      }
+      const float L = head_sum[hg * slices], inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+      const size_t head = static_cast<size_t>(r.b) * p.nq + h0 + hg;
+      *reinterpret_cast<uint2 *>(p.out + head * D + 4 * d) =
+          make_uint2(T::pack(o.x * inv, o.y * inv), T::pack(o.z * inv, o.w * inv));
+    }
+    return;
   }
-}
-
-// scores_out[b][kvh][n] = scores[b][kvh][n] + sum over the KV head's query heads of p_hn, n < lens[b].
-struct WeightParams {
-  const float *logits, *lse, *scores;
-  float *scores_out;
-  const int32_t *lens;
-  long long logit_row, in_seq, in_head, out_seq, out_head;  // strides, elements
-  int nq, group, max_len;
-};
-__global__ void __launch_bounds__(256) row_weight_kernel(const __grid_constant__ WeightParams p) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const int h = blockIdx.y, b = blockIdx.z, n = min(p.lens[b], p.max_len);
-  for (int k = blockIdx.x * 1024 + threadIdx.x; k < min(n, (static_cast<int>(blockIdx.x) + 1) * 1024); k += 256) {
-    float w = 0.f;
-    for (int g = 0; g < p.group; ++g) {
-      const size_t head = static_cast<size_t>(b) * p.nq + h * p.group + g;
-      w += fast_exp2(p.logits[head * p.logit_row + k] - p.lse[head]);
+  // ---- row weights: scores_out[b][h][n] = scores[b][h][n] + sum over the head's queries of p_hn
+  const int id = blockIdx.x - grid, k0 = id % row_blocks * kWeightRows;
+  const int bh = id / row_blocks, h = bh % p.cache.nkv, b = bh / p.cache.nkv;
+  const int n = min(kWeightRows, seq_rows(p, b) - k0);
+  if (n <= 0) return;
+  constexpr int R = kWeightRows / kJoinThreads;
+  float w[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) w[i] = 0.f;
+  for (int u = 0; u < p.units_per_kv; ++u) {
+    const int hu = h * p.units_per_kv + u, heads = min(HU, p.group - u * HU);
+    const size_t head0 = static_cast<size_t>(b) * p.nq + h * p.group + u * HU;
+    const int2 span = p.span[static_cast<size_t>(b) * p.cache.nkv * p.units_per_kv + hu];
+    if (warp < heads) {
+      float lse;
+      if (span.y < 0) {
+        lse = p.lse[head0 + warp];
+      } else {
+        const float2 ml = joined_ml(p, span.x, span.y, warp, lane);
+        lse = ml.y == 0.f ? INFINITY : ml.x + log2f(ml.y);
+      }
+      if (lane == 0) head_sum[warp] = lse;
     }
-    p.scores_out[b * p.out_seq + h * p.out_head + k] = p.scores[b * p.in_seq + h * p.in_head + k] + w;
+    __syncthreads();
+    for (int g = 0; g < heads; ++g) {
+      const float *lg = p.logits + (head0 + g) * p.logit_row + k0;
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const int k = tid + i * kJoinThreads;
+        if (k < n) w[i] += fast_exp2(lg[k] - head_sum[g]);
+      }
+    }
+    __syncthreads();
+  }
+  const float *in = p.scores + b * p.in_seq + h * p.in_head + k0;
+  float *out = p.scores_out + b * p.out_seq + h * p.out_head + k0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int k = tid + i * kJoinThreads;
+    if (k < n) out[k] = in[k] + w[i];
   }
 }
 

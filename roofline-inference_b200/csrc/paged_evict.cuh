@@ -7,13 +7,15 @@
 // order, so "the last rows" means the same after the next eviction.
 #pragma once
 
+#include <cooperative_groups.h>
+
 #include "paged_cache.cuh"
 
 namespace rib {
 namespace paged {
 
 constexpr int kSelThreads = 1024, kSelWarps = kSelThreads / 32;
-constexpr int kSelBins = 256;
+constexpr int kSelBins = 2048;
 
 struct SelectParams {
   const float *scores;         // [B][nkv] rows, strides s_seq, s_head
@@ -32,138 +34,199 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One CTA per (KV head, sequence).  The threshold is found by a radix walk over the keys, 8 bits a
-// pass, most significant first: histogram of the candidates that match the prefix so far, then the
-// bin that holds the wanted rank.  A last pass writes the kept rows in order; each warp takes a
-// consecutive run of rows, so one scan over the warps' counts places them.
-__global__ void __launch_bounds__(kSelThreads) select_rows_kernel(const __grid_constant__ SelectParams p) {
-  __shared__ uint32_t hist[kSelBins];
+constexpr int kSelMostRows = 24576;  // rows that a CTA keeps in shared memory (two CTAs to an SM)
+static_assert(kSelMostRows <= 32 * kSelThreads, "a lane for each 32 rows of a warp's run");
+
+// One cluster per (KV head, sequence); CTA r of it takes the r-th part of the rows, a warp a
+// consecutive run of the part, 32 at a time, so the kept rows come out in order.
+//
+// The threshold, the key of the last row that stays, is found digit by digit, most significant first:
+// a histogram of the candidates that match the digits found so far, summed over the cluster through
+// distributed shared memory (each CTA sums a slice of the bins and hands it to all), then the bin that
+// holds the wanted rank.  The walk ends early when all of that bin stays, mostly after two of the three
+// digits.  The first digit is the sign, the exponent and two more bits: accumulated weights have few
+// exponents, and with 8 bits a digit their additions queue at a handful of bins.
+// kCached: the scores are read once, into shared memory; longer parts are read again for every digit.
+template <bool kCached>
+__global__ void __launch_bounds__(kSelThreads, 2) select_rows_kernel(const __grid_constant__ SelectParams p) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  extern __shared__ float cached[];
+  __shared__ uint32_t hist[2][kSelBins];  // own counts, the cluster's
+  __shared__ uint32_t warp_sum[kSelWarps];
   __shared__ int n_gt[kSelWarps], n_eq[kSelWarps];
-  __shared__ uint32_t pick_bin, pick_rank;
+  __shared__ int cta_gt, cta_eq;
+  __shared__ uint32_t pick_bin, pick_rank, pick_count;
   pdl_launch_dependents();
   pdl_wait();
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int ctas = cluster.num_blocks(), rank_in = cluster.block_rank();
+  const int h = blockIdx.x / ctas, b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int given = p.lens[b];
   const int n = min(max(given, 0), p.max_len);
-  if (tid == 0 && h == 0) {
+  if (tid == 0 && blockIdx.x == 0) {
     p.new_lens[b] = min(n, p.keep);
     if (given < 0 || given > p.max_len) atomicExch(&g_device_status, RIB_ECAPACITY);
   }
   const float *sc = p.scores + b * p.s_seq + h * p.s_head;
   int32_t *rows = p.rows + (static_cast<size_t>(b) * p.nkv + h) * p.keep;
   float *ns = p.new_scores ? p.new_scores + b * p.n_seq + h * p.n_head : nullptr;
-  if (n <= p.keep) {
-    for (int i = tid; i < p.keep; i += kSelThreads) rows[i] = i < n ? i : -1;
+  if (n <= p.keep) {  // the same for the whole cluster
+    for (int i = rank_in * kSelThreads + tid; i < p.keep; i += ctas * kSelThreads) rows[i] = i < n ? i : -1;
     if (ns)
-      for (int i = tid; i < p.new_width; i += kSelThreads) ns[i] = i < n ? sc[i] : 0.f;
+      for (int i = rank_in * kSelThreads + tid; i < p.new_width; i += ctas * kSelThreads) ns[i] = i < n ? sc[i] : 0.f;
     return;
   }
-  const int lo = p.sinks, hi = n - p.recent;        // candidates [lo, hi)
-  uint32_t rank = p.keep - p.sinks - p.recent;      // of which this many stay
-  uint32_t prefix = 0;                              // the key of the last one that stays
-  if (rank > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
-      __syncthreads();
-      const uint32_t high = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-      for (int i = lo + tid; i < hi; i += kSelThreads) {
-        const uint32_t key = order_key(sc[i]);
-        if ((key & high) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
+  // this CTA's part of the rows, and of it each warp's run of `per` times 32 rows
+  const int per = (n + ctas * kSelThreads - 1) / (ctas * kSelThreads), part = per * kSelThreads;
+  const int base = min(rank_in * part, n), mine = min(part, n - base);
+  const float *from = sc + base;
+  if (kCached) {
+    for (int i = tid; i < mine; i += kSelThreads)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(cached + i)), "l"(from + i) : "memory");
+    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+    from = cached;
+  }
+  for (int i = tid; i < kSelBins; i += kSelThreads) hist[0][i] = 0;
+  __syncthreads();
+  const int lo = p.sinks - base, hi = n - p.recent - base;      // candidates [lo, hi) of the part
+  const uint32_t stay = p.keep - p.sinks - p.recent;            // of all candidates, this many stay
+  uint32_t rank = stay, prefix = 0, known = 0;                  // `known`: the bits of the key found so far
+  if (stay > 0) {
+#pragma unroll 1
+    for (int digit = 0; digit < 3; ++digit) {
+      const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
+      const uint32_t bits = digit == 2 ? 1023u : 2047u;
+      for (int i = max(lo, 0) + tid; i < min(hi, mine); i += kSelThreads) {
+        const uint32_t key = order_key(from[i]);
+        if ((key & known) == prefix) atomicAdd(&hist[0][(key >> shift) & bits], 1u);
       }
-      __syncthreads();
-      if (warp == 0) {  // lane holds 8 bins, highest bins in lane 0: counts from the top
-        uint32_t c[8], sum = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          c[j] = hist[255 - (8 * lane + j)];
-          sum += c[j];
+      const uint32_t *total = hist[0];
+      if (ctas > 1) {
+        cluster.sync();
+        const int slice = kSelBins / ctas;  // 2, 4 or 8 CTAs
+        for (int i = tid; i < slice; i += kSelThreads) {
+          const int bin = rank_in * slice + i;
+          uint32_t sum = 0;
+          for (int r = 0; r < ctas; ++r) sum += cluster.map_shared_rank(hist[0], r)[bin];
+          for (int r = 0; r < ctas; ++r) cluster.map_shared_rank(hist[1], r)[bin] = sum;
         }
-        uint32_t inc = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
-          if (lane >= o) inc += up;
-        }
-        uint32_t above = inc - sum;
-        if (above < rank && rank <= inc) {
-          for (int j = 0; j < 8; ++j) {
-            if (rank <= above + c[j]) {
-              pick_bin = 255 - (8 * lane + j);
-              pick_rank = rank - above;
-              break;
-            }
-            above += c[j];
-          }
-        }
+        cluster.sync();
+        total = hist[1];
+      } else {
+        __syncthreads();
       }
+      // two bins a thread, from the highest down: their counts, then those above
+      const uint2 u = reinterpret_cast<const uint2 *>(total)[kSelBins / 2 - 1 - tid];
+      uint32_t inc = u.x + u.y;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += up;
+      }
+      if (lane == 31) warp_sum[warp] = inc;
+      __syncthreads();
+      const uint32_t above = inc - (u.x + u.y) + __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0u);
+      if (above < rank && rank <= above + u.x + u.y) {
+        const bool second = rank > above + u.y;
+        pick_bin = kSelBins - 1 - 2 * tid - second;
+        pick_rank = rank - above - (second ? u.y : 0);
+        pick_count = second ? u.x : u.y;
+      }
+      for (int i = tid; i < kSelBins; i += kSelThreads) hist[0][i] = 0;
       __syncthreads();
       prefix |= pick_bin << shift;
-      rank = pick_rank;  // rank within the bin; after the last pass: how many equal keys stay
-      __syncthreads();
+      known |= bits << shift;
+      rank = pick_rank;  // within the bin: at the end, how many of the rows that match the prefix stay
+      if (rank == pick_count) break;
     }
   }
-  const bool any = p.keep - p.sinks - p.recent > 0;
-  const int ties = any ? static_cast<int>(rank) : 0;
-  // ---- ordered write: class 2 stays for certain, class 1 equals the threshold
-  const int per = (n + kSelThreads - 1) / kSelThreads * 32;  // rows of a warp
-  const int w_lo = min(warp * per, n), w_hi = min(w_lo + per, n);
+  const int ties = static_cast<int>(rank);
+  // ---- ordered write: class 2 stays for certain, class 1 matches the threshold
+  const int w_lo = warp * per * 32;
   auto cls = [&](int i) {
-    if (i >= w_hi) return 0;
+    if (i >= mine) return 0;
     if (i < lo || i >= hi) return 2;
-    if (!any) return 0;
-    const uint32_t key = order_key(sc[i]);
+    if (stay == 0) return 0;
+    const uint32_t key = order_key(from[i]) & known;
     return key > prefix ? 2 : key == prefix ? 1 : 0;
   };
+  // lane v keeps the classes of the run's v-th 32 rows (with 32 of those at most)
+  uint32_t kept_gt = 0, kept_eq = 0;
   int gt = 0, eq = 0;
-  for (int i = w_lo; i < w_hi; i += 32) {
-    const int k = cls(i + lane);
-    gt += __popc(__ballot_sync(0xffffffffu, k == 2));
-    eq += __popc(__ballot_sync(0xffffffffu, k == 1));
+  for (int v = 0; v < per; ++v) {
+    const int k = cls(w_lo + v * 32 + lane);
+    const uint32_t mg = __ballot_sync(0xffffffffu, k == 2), me = __ballot_sync(0xffffffffu, k == 1);
+    gt += __popc(mg);
+    eq += __popc(me);
+    if (kCached && lane == v) {
+      kept_gt = mg;
+      kept_eq = me;
+    }
   }
   if (lane == 0) {
     n_gt[warp] = gt;
     n_eq[warp] = eq;
   }
   __syncthreads();
-  int g0 = 0, e0 = 0;
-  for (int w = 0; w < warp; ++w) {
-    g0 += n_gt[w];
-    e0 += n_eq[w];
+  int g0 = __reduce_add_sync(0xffffffffu, lane < warp ? n_gt[lane] : 0);
+  int e0 = __reduce_add_sync(0xffffffffu, lane < warp ? n_eq[lane] : 0);
+  if (ctas > 1) {
+    if (tid == kSelThreads - 1) {
+      cta_gt = g0 + gt;
+      cta_eq = e0 + eq;
+    }
+    cluster.sync();
+    const int other = lane < rank_in ? lane : rank_in;
+    g0 += __reduce_add_sync(0xffffffffu, lane < rank_in ? *cluster.map_shared_rank(&cta_gt, other) : 0);
+    e0 += __reduce_add_sync(0xffffffffu, lane < rank_in ? *cluster.map_shared_rank(&cta_eq, other) : 0);
   }
-  const uint32_t below = (1u << lane) - 1;
-  for (int i = w_lo; i < w_hi; i += 32) {
-    const int k = cls(i + lane);
-    const uint32_t mg = __ballot_sync(0xffffffffu, k == 2), me = __ballot_sync(0xffffffffu, k == 1);
-    const int e = e0 + __popc(me & below), g = g0 + __popc(mg & below);
-    if (k == 2 || (k == 1 && e < ties)) {
-      const int at = g + min(e, ties);
-      rows[at] = i + lane;
-      if (ns) ns[at] = sc[i + lane];
+  const uint32_t below = (1u << lane) - 1, bit = 1u << lane;
+#pragma unroll 2
+  for (int v = 0; v < per; ++v) {
+    const int i = w_lo + v * 32 + lane;
+    uint32_t mg, me;
+    if (kCached) {
+      mg = __shfl_sync(0xffffffffu, kept_gt, v);
+      me = __shfl_sync(0xffffffffu, kept_eq, v);
+    } else {
+      const int k = cls(i);
+      mg = __ballot_sync(0xffffffffu, k == 2);
+      me = __ballot_sync(0xffffffffu, k == 1);
+    }
+    const int e = e0 + __popc(me & below);
+    if ((mg & bit) || ((me & bit) && e < ties)) {
+      const int at = g0 + __popc(mg & below) + min(e, ties);
+      rows[at] = base + i;
+      if (ns) ns[at] = from[i];
     }
     g0 += __popc(mg);
     e0 += __popc(me);
   }
   if (ns)
-    for (int i = p.keep + tid; i < p.new_width; i += kSelThreads) ns[i] = 0.f;
+    for (int i = p.keep + rank_in * kSelThreads + tid; i < p.new_width; i += ctas * kSelThreads) ns[i] = 0.f;
+  if (ctas > 1) cluster.sync();  // no CTA leaves while another may read its counts
 }
 
 // Moves the kept rows: row j of the new table's sequence gets row rows[j] of the old one, K and V.
 struct MoveParams {
   View from, to;               // the same pages through two tables
   const int32_t *rows;         // [B][nkv][keep]
-  int keep, dim;
+  int keep;
 };
 
-// A warp takes 32 kept rows of one KV head: each lane looks one row's two pages up, then 16-byte
-// pieces move, K and V of 2 * D / 8 lanes to a row.
-__global__ void __launch_bounds__(256) move_rows_kernel(const __grid_constant__ MoveParams p) {
+// A warp takes kMoveRows kept rows of one KV head: a lane each looks one row's two pages up, then the
+// rows move in 16-byte pieces, K and V of 2 * D / 8 lanes to a row, all loads before the first store.
+constexpr int kMoveRows = 8, kMoveThreads = 256;
+
+template <int D>
+__global__ void __launch_bounds__(kMoveThreads) move_rows_kernel(const __grid_constant__ MoveParams p) {
   pdl_launch_dependents();
   pdl_wait();
   const int h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31;
-  const int j0 = (blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32) * 32;
+  const int j0 = (blockIdx.x * (kMoveThreads / 32) + threadIdx.x / 32) * kMoveRows;
   if (j0 >= p.keep) return;
   const int j = j0 + lane;
-  const int r = j < p.keep ? p.rows[(static_cast<size_t>(b) * p.from.nkv + h) * p.keep + j] : -1;
+  const int r = lane < kMoveRows && j < p.keep ? p.rows[(static_cast<size_t>(b) * p.from.nkv + h) * p.keep + j] : -1;
   long long src = -1, dst = -1;
   if (r >= 0) {
     const int a = page_of(p.from, b, r), z = page_of(p.to, b, j);
@@ -174,15 +237,19 @@ __global__ void __launch_bounds__(256) move_rows_kernel(const __grid_constant__ 
       atomicExch(&g_device_status, RIB_ECAPACITY);
     }
   }
-  const int vec = p.dim / 8, lanes = 2 * vec;  // 16-byte pieces of a K row; lanes of a row (32, 16)
-  const int side = lane / lanes, piece = lane % lanes;
-  const long long off = (piece >= vec ? p.from.s_half : 0) + (piece % vec) * 8;
-  const int step = 32 / lanes;
-#pragma unroll 8
-  for (int i = 0; i < 32; i += step) {
-    const long long s = __shfl_sync(0xffffffffu, src, i + side), d = __shfl_sync(0xffffffffu, dst, i + side);
-    if (s >= 0)
-      *reinterpret_cast<uint4 *>(p.to.pages + d + off) = *reinterpret_cast<const uint4 *>(p.from.pages + s + off);
+  constexpr int V = D / 8, L = 2 * V, S = 32 / L;  // pieces of a K row; lanes of a row; rows of a step
+  const int side = lane / L, piece = lane % L;
+  const long long off = (piece >= V ? p.from.s_half : 0) + (piece % V) * 8;
+  uint4 x[kMoveRows / S];
+#pragma unroll
+  for (int i = 0; i < kMoveRows / S; ++i) {
+    const long long s = __shfl_sync(0xffffffffu, src, i * S + side);
+    if (s >= 0) x[i] = *reinterpret_cast<const uint4 *>(p.from.pages + s + off);
+  }
+#pragma unroll
+  for (int i = 0; i < kMoveRows / S; ++i) {
+    const long long d = __shfl_sync(0xffffffffu, dst, i * S + side);
+    if (d >= 0) *reinterpret_cast<uint4 *>(p.to.pages + d + off) = x[i];
   }
 }
 
