@@ -1,4 +1,5 @@
-"""Loader of the C-ABI library librib_attention.so (CUDA kernels for sm_100a).
+"""Loader of the C-ABI library librib_attention.so (CUDA kernels for sm_100a), and of the native Python
+binding of its paged-cache entry points (_paged_binding.so).
 
 The library is built in-tree from csrc/ with nvcc.  `load()` rebuilds it when
 the sources changed (content hash, not mtimes, so a copied tree is recognised
@@ -11,9 +12,11 @@ from __future__ import annotations
 import ctypes
 import fcntl
 import hashlib
+import importlib.util
 import os
 import shutil
 import subprocess
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -23,6 +26,9 @@ HEADER = REPO_DIR / "include" / "rib_attention.h"
 LIB_PATH = PKG_DIR / "librib_attention.so"
 STAMP = PKG_DIR / "librib_attention.so.srchash"
 MAIN_SOURCE = CSRC / "rib_attention.cu"
+BINDING_SOURCE = CSRC / "paged_binding.cpp"
+BINDING_PATH = PKG_DIR / "_paged_binding.so"
+BINDING_STAMP = PKG_DIR / "_paged_binding.so.srchash"
 
 EXPORTS = CSRC / "exports.map"
 NVCC_FLAGS = [
@@ -36,6 +42,7 @@ NVCC_FLAGS = [
 RIB_OK, RIB_EINVAL, RIB_ECAPACITY, RIB_EALIGN, RIB_ECUDA, RIB_ETIMEOUT = range(6)
 
 _lib: ctypes.CDLL | None = None
+_binding_module = None
 
 
 def _sources() -> list[Path]:
@@ -62,30 +69,61 @@ def _nvcc() -> str:
     raise RuntimeError("nvcc not found: cannot build librib_attention.so")
 
 
+def _run(cmd: list[str], tool: str, verbose: bool) -> None:
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{tool} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+    if verbose:
+        print(res.stdout + res.stderr)
+
+
+def _binding_command() -> list[str]:
+    import torch
+    root = Path(torch.__file__).parent
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+            f"-I{sysconfig.get_paths()['include']}", f"-I{root / 'include'}",
+            f"-I{root / 'include/torch/csrc/api/include'}", f"-I{Path(_nvcc()).resolve().parent.parent / 'include'}",
+            str(BINDING_SOURCE), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+
+
+def binding_hash() -> str:
+    import torch
+    h = hashlib.sha256(f"{torch.__version__} {sysconfig.get_python_version()}".encode())
+    for p in (BINDING_SOURCE, HEADER):
+        h.update(p.read_bytes())
+    return h.hexdigest()
+
+
+def binding_is_current() -> bool:
+    return BINDING_PATH.exists() and BINDING_STAMP.exists() and BINDING_STAMP.read_text().strip() == binding_hash()
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compiles csrc/rib_attention.cu for sm_100a into librib_attention.so.
+    """Compiles csrc/rib_attention.cu for sm_100a into librib_attention.so, and
+    csrc/paged_binding.cpp against this process's torch into _paged_binding.so.
 
     Serialised with a file lock so that several ranks importing the package at
-    once build it only once."""
-    if not force and is_current():
+    once build them only once."""
+    if not force and is_current() and binding_is_current():
         return LIB_PATH
     lock_path = PKG_DIR / ".librib_attention.lock"
     with open(lock_path, "w") as lock:
         fcntl.flock(lock, fcntl.LOCK_EX)
         try:
-            if not force and is_current():
-                return LIB_PATH
-            tmp = LIB_PATH.with_name(f"{LIB_PATH.name}.{os.getpid()}.tmp")
-            cmd = [_nvcc(), *NVCC_FLAGS, "-o", str(tmp), str(MAIN_SOURCE)]
-            if verbose:
-                cmd.insert(1, "-Xptxas=-v")
-            res = subprocess.run(cmd, capture_output=True, text=True)
-            if res.returncode != 0:
-                raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
-            if verbose:
-                print(res.stdout + res.stderr)
-            tmp.replace(LIB_PATH)
-            STAMP.write_text(source_hash() + "\n")
+            if force or not is_current():
+                tmp = LIB_PATH.with_name(f"{LIB_PATH.name}.{os.getpid()}.tmp")
+                cmd = [_nvcc(), *NVCC_FLAGS, "-o", str(tmp), str(MAIN_SOURCE)]
+                if verbose:
+                    cmd.insert(1, "-Xptxas=-v")
+                _run(cmd, "nvcc", verbose)
+                tmp.replace(LIB_PATH)
+                STAMP.write_text(source_hash() + "\n")
+            if force or not binding_is_current():
+                tmp = BINDING_PATH.with_name(f"{BINDING_PATH.name}.{os.getpid()}.tmp")
+                _run([*_binding_command(), "-o", str(tmp)], "g++", verbose)
+                tmp.replace(BINDING_PATH)
+                BINDING_STAMP.write_text(binding_hash() + "\n")
         finally:
             fcntl.flock(lock, fcntl.LOCK_UN)
     return LIB_PATH
@@ -150,6 +188,21 @@ def load() -> ctypes.CDLL:
         _bind(L)
         _lib = L
     return _lib
+
+
+def binding():
+    """The native binding of the paged-cache entry points (once per process)."""
+    global _binding_module
+    if _binding_module is None:
+        L = load()
+        spec = importlib.util.spec_from_file_location("_paged_binding", BINDING_PATH)
+        m = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(m)
+        m.bind(*(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in (
+            "rib_status_string", "rib_last_error_string", "rib_rotary_apply", "rib_paged_append",
+            "rib_paged_decode_workspace_bytes", "rib_paged_decode_attention", "rib_paged_evict")))
+        _binding_module = m
+    return _binding_module
 
 
 def check(status: int, what: str) -> None:

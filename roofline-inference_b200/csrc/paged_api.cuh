@@ -155,11 +155,18 @@ int paged_decode_launch(const rib::paged::DecodeParams &p, int grid, cudaStream_
     return rib::host_fail(RIB_ECUDA, "cudaFuncSetAttribute(paged decode smem)", smem);
   const int s = launch_pdl("paged_decode_kernel launch", kernel, dim3(grid), dim3(NT), smem, st, p);
   if (s != RIB_OK) return s;
-  const int row_blocks = kLogits ? ceil_div(p.max_len, kWeightRows) : 0;
-  const long long blocks = grid + static_cast<long long>(row_blocks) * p.cache.nkv * p.batch;
+  // blocks of row weights: enough to fill the GPU once, of 1024 rows at least
+  const long long heads = static_cast<long long>(p.cache.nkv) * p.batch, room = 4LL * sm_count();
+  int row_blocks = 0, rows = 0;
+  if (kLogits) {
+    rows = ceil_div(p.max_len, std::min<long long>(ceil_div(p.max_len, 1024), ceil_div(room, std::min(heads, room))));
+    rows = ceil_div(rows, 1024) * 1024;
+    row_blocks = ceil_div(p.max_len, rows);
+  }
+  const long long blocks = grid + row_blocks * heads;
   if (blocks > 0x7fffffffLL) return RIB_EINVAL;
   return launch_pdl("join_kernel launch", join_kernel<T, D>, dim3(static_cast<unsigned>(blocks)), dim3(kJoinThreads), 0,
-                    st, p, grid, row_blocks);
+                    st, p, grid, row_blocks, rows);
 }
 
 template <class T>
@@ -270,8 +277,6 @@ int rib_paged_decode_attention(const rib_paged_cache *cache, const void *q, long
   if (!q || !lens || !out || batch < 1 || batch > cache->seqs || nq < 1 || nq % cache->nkv || max_len < 1 ||
       max_len > static_cast<long long>(cache->width) * cache->page_rows || !(scale > 0.f) || !(scale < INFINITY) ||
       (dim != 64 && dim != 128) || cache->page_rows % TK || !scores != !scores_out)
-    return RIB_EINVAL;
-  if (scores && static_cast<long long>(batch) * cache->nkv * ceil_div(max_len, kWeightRows) > 0x7fff0000LL)
     return RIB_EINVAL;
   const PagedDecodeLayout l = paged_decode_layout(batch, max_len, nq, dim, scores != nullptr);
   if (!workspace || workspace_bytes < l.total) return RIB_EINVAL;

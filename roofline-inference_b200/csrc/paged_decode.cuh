@@ -47,7 +47,8 @@ struct DecodeCfg {
 template <int D>
 struct DecodeSmem {
   alignas(1024) uint8_t ring[NW][DecodeCfg<D>::ST][DecodeCfg<D>::STAGE];
-  alignas(16) float o[NW - 1][HU][D];
+  // [warp that sums][the others][head][its share of the dims], rows padded against bank conflicts
+  alignas(16) float o[NW][NW - 1][HU][D / NW + 8];
   float m[NW][HU], l[NW][HU];
   uint64_t full[NW][DecodeCfg<D>::ST];
   long long sum[NW];                              // tiles of each warp's sequences
@@ -386,48 +387,52 @@ __global__ void __launch_bounds__(NT, kCtasPerSm) paged_decode_kernel(const __gr
     for (int w = 1; w < NW; ++w) M = fmaxf(M, sm.m[w][g]);
     const float al = M == -INFINITY ? 0.f : fast_exp2(m - M);
     if (t4 == 0) sm.l[warp][g] = l * al;
+    // every warp sums a share of the dims: it keeps its own part of those and hands out the rest
+    constexpr int S = D / 8 / NW;  // n-tiles of a share
+    float2 own[S];
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) {
-      o[i][0] = (o[i][0] + o[i][2]) * al;
-      o[i][1] = (o[i][1] + o[i][3]) * al;
-      if (warp > 0) *reinterpret_cast<float2 *>(&sm.o[warp - 1][g][8 * i + 2 * t4]) = make_float2(o[i][0], o[i][1]);
+      const float2 v = make_float2((o[i][0] + o[i][2]) * al, (o[i][1] + o[i][3]) * al);
+      if (i / S == warp)
+        own[i % S] = v;
+      else
+        *reinterpret_cast<float2 *>(&sm.o[i / S][warp - (warp > i / S)][g][i % S * 8 + 2 * t4]) = v;
     }
     __syncthreads();
-    if (warp == 0) {
+    {
       float L = sm.l[0][g];
 #pragma unroll
       for (int w = 1; w < NW; ++w) L += sm.l[w][g];
       const bool whole = c.tile == 0 && seg == c.tiles;
       const int part = c.tile > 0 ? 0 : 1;
-      const float inv = whole ? (L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L)) : 1.f;  // a NaN sum stays NaN
-      float *po = p.part_o + (static_cast<size_t>(cta) * 2 + part) * HU * D + g * D;
+      const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);  // a NaN sum stays NaN
+      const int d0 = warp * (D / NW) + 2 * t4;
+      uint16_t *out = p.out + (static_cast<size_t>(c.b) * p.nq + h0 + g) * D + d0;
+      float *po = p.part_o + ((static_cast<size_t>(cta) * 2 + part) * HU + g) * D + d0;
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        float2 v = make_float2(o[i][0], o[i][1]);
+      for (int i = 0; i < S; ++i) {
+        float2 v = make_float2(0.f, 0.f);  // in warp order
 #pragma unroll
-        for (int w = 0; w < NW - 1; ++w) {
-          const float2 u = *reinterpret_cast<const float2 *>(&sm.o[w][g][8 * i + 2 * t4]);
+        for (int w = 0; w < NW; ++w) {
+          const float2 u = w == warp ? own[i]
+                                     : *reinterpret_cast<const float2 *>(&sm.o[warp][w - (w > warp)][g][i * 8 + 2 * t4]);
           v.x += u.x;
           v.y += u.y;
         }
         if (g < heads) {
           if (whole)
-            *reinterpret_cast<uint32_t *>(p.out + (static_cast<size_t>(c.b) * p.nq + h0 + g) * D + 8 * i + 2 * t4) =
-                T::pack(v.x * inv, v.y * inv);
+            *reinterpret_cast<uint32_t *>(out + 8 * i) = T::pack(v.x * inv, v.y * inv);
           else
-            *reinterpret_cast<float2 *>(po + 8 * i + 2 * t4) = v;
+            *reinterpret_cast<float2 *>(po + 8 * i) = v;
         }
       }
-      if (t4 == 0 && g < heads) {
-        if (!whole) {
-          float *ml = p.part_ml + ((static_cast<size_t>(cta) * 2 + part) * HU + g) * 2;
-          ml[0] = M;
-          ml[1] = L;
-        } else if (kLogits) {
+      if (warp == 0 && t4 == 0 && g < heads) {
+        if (!whole)
+          *reinterpret_cast<float2 *>(p.part_ml + ((static_cast<size_t>(cta) * 2 + part) * HU + g) * 2) = make_float2(M, L);
+        else if (kLogits)
           p.lse[static_cast<size_t>(c.b) * p.nq + h0 + g] = L == 0.f ? INFINITY : M + log2f(L);
-        }
       }
-      if (lane == 0) {
+      if (tid == 0) {
         int last = -1;  // the CTA in which a unit that begins here and does not end here ends
         if (c.tile == 0 && !whole) {
           const long long x = s0 + f + c.tiles - 1, big = rest * (quot + 1);  // its last tile
@@ -447,7 +452,6 @@ __global__ void __launch_bounds__(NT, kCtasPerSm) paged_decode_kernel(const __gr
 }
 
 constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * 32;
-constexpr int kWeightRows = 1024;  // rows of a weight block
 
 // Place of CTA c's partial of a unit that begins in CTA `first`: that one's second, the others' first.
 __device__ __forceinline__ size_t part_slot(int c, int first) { return static_cast<size_t>(c) * 2 + (c == first); }
@@ -474,10 +478,10 @@ __device__ __forceinline__ float2 joined_ml(const DecodeParams &p, int first, in
 
 // Blocks below `grid`: join the unit that begins in that CTA's run and ends in another's.  The warps
 // take (head, slice of the partials), so all partials are under way at once; the slices are summed in
-// order.  With scores, the blocks behind add the row weights of kWeightRows rows of one KV head each.
+// order.  With scores, the blocks behind add the row weights, `rows` rows of one KV head each.
 template <class T, int D>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ DecodeParams p, int grid,
-                                                            int row_blocks) {
+                                                            int row_blocks, int rows) {
   __shared__ float4 acc[kJoinWarps][D / 4];
   __shared__ float head_sum[kJoinWarps];
   pdl_launch_dependents();
@@ -490,19 +494,32 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     const int heads = min(HU, p.group - g0), h0 = kvh * p.group + g0;
     const int slices = kJoinWarps / heads, g = warp / slices, slice = warp % slices;
     constexpr int V = D / 4, R = 32 / V;  // lanes of a row, rows of a load
-    const int v = lane % V, sub = lane / V;
+    constexpr int N = D == 128 ? 6 : 4;   // loads under way at once
+    const int v = lane % V, step = slices * R;
     if (g < heads) {
-      const float2 ml = joined_ml(p, first, r.last, g, lane);
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int c = first + slice * R + sub; c <= r.last; c += slices * R) {
-        const size_t s = part_slot(c, first) * HU + g;
-        const float4 u = *reinterpret_cast<const float4 *>(p.part_o + s * D + 4 * v);
-        const float al = ml.x == -INFINITY ? 0.f : fast_exp2(p.part_ml[2 * s] - ml.x);
-        o.x = fmaf(u.x, al, o.x);
-        o.y = fmaf(u.y, al, o.y);
-        o.z = fmaf(u.z, al, o.z);
-        o.w = fmaf(u.w, al, o.w);
+      float2 all = make_float2(0.f, 0.f);
+      for (int c0 = first + slice * R + lane / V; c0 - lane / V <= r.last; c0 += N * step) {
+        float4 u[N];
+        float m[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int c = c0 + i * step;
+          if (c > r.last) continue;
+          const size_t s = part_slot(c, first) * HU + g;
+          u[i] = *reinterpret_cast<const float4 *>(p.part_o + s * D + 4 * v);
+          m[i] = p.part_ml[2 * s];
+        }
+        if (c0 - lane / V == first + slice * R) all = joined_ml(p, first, r.last, g, lane);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (c0 + i * step > r.last) continue;
+          const float al = all.x == -INFINITY ? 0.f : fast_exp2(m[i] - all.x);
+          o.x = fmaf(u[i].x, al, o.x);
+          o.y = fmaf(u[i].y, al, o.y);
+          o.z = fmaf(u[i].z, al, o.z);
+          o.w = fmaf(u[i].w, al, o.w);
+        }
       }
       if (R == 2) {
         o.x += __shfl_xor_sync(0xffffffffu, o.x, 16);
@@ -510,8 +527,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
         o.z += __shfl_xor_sync(0xffffffffu, o.z, 16);
         o.w += __shfl_xor_sync(0xffffffffu, o.w, 16);
       }
-      if (sub == 0) acc[warp][v] = o;
-      if (lane == 0) head_sum[warp] = ml.y;
+      if (lane < V) acc[warp][v] = o;
+      if (lane == 0 && slice == 0) head_sum[g] = all.y;
     }
     __syncthreads();
     for (int i = tid; i < heads * V; i += kJoinThreads) {
@@ -521,7 +538,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
         const float4 u = acc[hg * slices + k][d];
         o = make_float4(o.x + u.x, o.y + u.y, o.z + u.z, o.w + u.w);
       }
-      const float L = head_sum[hg * slices], inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+      const float L = head_sum[hg], inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
       const size_t head = static_cast<size_t>(r.b) * p.nq + h0 + hg;
       *reinterpret_cast<uint2 *>(p.out + head * D + 4 * d) =
           make_uint2(T::pack(o.x * inv, o.y * inv), T::pack(o.z * inv, o.w * inv));
@@ -529,19 +546,16 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     return;
   }
   // ---- row weights: scores_out[b][h][n] = scores[b][h][n] + sum over the head's queries of p_hn
-  const int id = blockIdx.x - grid, k0 = id % row_blocks * kWeightRows;
+  const int id = blockIdx.x - grid, k0 = id % row_blocks * rows;
   const int bh = id / row_blocks, h = bh % p.cache.nkv, b = bh / p.cache.nkv;
-  const int n = min(kWeightRows, seq_rows(p, b) - k0);
+  const int n = min(rows, seq_rows(p, b) - k0);
   if (n <= 0) return;
-  constexpr int R = kWeightRows / kJoinThreads;
-  float w[R];
-#pragma unroll
-  for (int i = 0; i < R; ++i) w[i] = 0.f;
+  float *out = p.scores_out + b * p.out_seq + h * p.out_head + k0;
   for (int u = 0; u < p.units_per_kv; ++u) {
     const int hu = h * p.units_per_kv + u, heads = min(HU, p.group - u * HU);
     const size_t head0 = static_cast<size_t>(b) * p.nq + h * p.group + u * HU;
-    const int2 span = p.span[static_cast<size_t>(b) * p.cache.nkv * p.units_per_kv + hu];
     if (warp < heads) {
+      const int2 span = p.span[static_cast<size_t>(b) * p.cache.nkv * p.units_per_kv + hu];
       float lse;
       if (span.y < 0) {
         lse = p.lse[head0 + warp];
@@ -552,22 +566,32 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
       if (lane == 0) head_sum[warp] = lse;
     }
     __syncthreads();
-    for (int g = 0; g < heads; ++g) {
-      const float *lg = p.logits + (head0 + g) * p.logit_row + k0;
+    const float *in = u ? out : p.scores + b * p.in_seq + h * p.in_head + k0;
+    constexpr int R = 4;
+    for (int k = tid; k < n; k += R * kJoinThreads) {
+      float x[HU][R], w[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i) w[i] = k + i * kJoinThreads < n ? in[k + i * kJoinThreads] : 0.f;
+#pragma unroll
+      for (int g = 0; g < HU; ++g)
+        if (g < heads) {
+          const float *lg = p.logits + (head0 + g) * p.logit_row + k0 + k;
+#pragma unroll
+          for (int i = 0; i < R; ++i) x[g][i] = k + i * kJoinThreads < n ? lg[i * kJoinThreads] : -INFINITY;
+        }
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        const int k = tid + i * kJoinThreads;
-        if (k < n) w[i] += fast_exp2(lg[k] - head_sum[g]);
+        float sum = 0.f;
+#pragma unroll
+        for (int g = 0; g < HU; ++g)
+          if (g < heads) sum += fast_exp2(x[g][i] - head_sum[g]);
+        w[i] += sum;
       }
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        if (k + i * kJoinThreads < n) out[k + i * kJoinThreads] = w[i];
     }
     __syncthreads();
-  }
-  const float *in = p.scores + b * p.in_seq + h * p.in_head + k0;
-  float *out = p.scores_out + b * p.out_seq + h * p.out_head + k0;
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int k = tid + i * kJoinThreads;
-    if (k < n) out[k] = in[k] + w[i];
   }
 }
 
