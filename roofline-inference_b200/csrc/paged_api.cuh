@@ -106,7 +106,7 @@ struct PagedDecodeLayout {
 PagedDecodeLayout paged_decode_layout(int batch, int max_len, int nq, int dim, bool scores) {
   using namespace rib::paged;
   PagedDecodeLayout l;
-  l.grid = kCtasPerSm * sm_count();
+  l.grid = (dim == 128 ? DecodeCfg<128>::CTAS : DecodeCfg<64>::CTAS) * sm_count();
   size_t off = round256(static_cast<size_t>(l.grid) * 2 * HU * dim * sizeof(float));
   l.ml_off = off;
   off += round256(static_cast<size_t>(l.grid) * 2 * HU * 2 * sizeof(float));

@@ -34,12 +34,12 @@ constexpr int TK = 16;        // rows of a tile: one TMA box, one page at most
 constexpr int NW = 4;         // warps of a CTA
 constexpr int NT = NW * 32;
 constexpr int HU = 8;         // query heads of a unit
-constexpr int kCtasPerSm = 2;
 constexpr int kMinTiles = 8;  // fewest tiles of a CTA's run while other CTAs idle
 
 template <int D>
 struct DecodeCfg {
-  static constexpr int ST = 384 / D;              // ring slots of a warp: 24 KB in flight
+  static constexpr int CTAS = D == 128 ? 2 : 3;   // resident per SM
+  static constexpr int ST = D == 128 ? 2 : 3;     // ring slots of a warp
   static constexpr int HALF = 2 * TK * 128;       // bytes of one box: 64 dims of K and of V rows
   static constexpr int STAGE = HALF * (D / 64);
 };
@@ -84,12 +84,19 @@ struct DecodeParams {
 };
 
 __device__ __forceinline__ void tma_load_5d(void *dst, const void *tmap, int c0, int c1, int c2, int c3, int c4,
-                                            uint64_t *bar) {
+                                            uint64_t *bar, uint64_t policy) {
   asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(smem_u32(bar))
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7], %8;" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(smem_u32(bar)),
+      "l"(policy)
       : "memory");
+}
+
+__device__ __forceinline__ uint64_t l2_policy_evict_normal() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
+  return p;
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -147,7 +154,7 @@ __device__ __forceinline__ bool next_unit(const DecodeParams &p, Place &c, int u
 }
 
 template <class T, int D, bool kLogits>
-__global__ void __launch_bounds__(NT, kCtasPerSm) paged_decode_kernel(const __grid_constant__ DecodeParams p) {
+__global__ void __launch_bounds__(NT, DecodeCfg<D>::CTAS) paged_decode_kernel(const __grid_constant__ DecodeParams p) {
   using Cfg = DecodeCfg<D>;
   constexpr int ST = Cfg::ST;
   extern __shared__ uint8_t smem_raw[];
@@ -229,6 +236,7 @@ __global__ void __launch_bounds__(NT, kCtasPerSm) paged_decode_kernel(const __gr
 
   // ---- producer side of the warp: tile i of the warp is the run's tile warp + i * NW
   const int count = run > warp ? (run - warp + NW - 1) / NW : 0;
+  const uint64_t policy = p.units_per_kv == 1 ? l2_policy_evict_first() : l2_policy_evict_normal();
   // moves `by` tiles along the run
   auto seek = [&](Place &pl, int by) {
     pl.tile += by;
@@ -250,7 +258,7 @@ __global__ void __launch_bounds__(NT, kCtasPerSm) paged_decode_kernel(const __gr
 #pragma unroll
     for (int hf = 0; hf < D / 64; ++hf)
       tma_load_5d(sm.ring[warp][slot] + hf * Cfg::HALF, &p.map, 64 * hf, pl.tile * TK % p.cache.page_rows,
-                  pl.hu / p.units_per_kv, 0, page, &sm.full[warp][slot]);
+                  pl.hu / p.units_per_kv, 0, page, &sm.full[warp][slot], policy);
   };
   if (lane < min(ST, count)) {  // the first tiles, a lane each
     Place pl = c;
