@@ -19,6 +19,7 @@ from .kernels import (add_rms, argmax, embedding, gemv, qk_norm_rope, qk_norm_ro
 from .model import QWEN3_0_6B, DecodeGraph, Engine, Qwen3Config, Qwen3Weights, random_weights
 from .batch import BatchDecoder, SlotDecoder, generate_batch
 from .paged import Rotary, paged_append, paged_decode_attention, paged_evict, rotary
+from .paged_batch import PagedDecoder, PagePool
 from .pool import KVPool, PoolFull
 from .scheduler import Request, Scheduler
 
@@ -28,6 +29,8 @@ __all__ = [
     "DecodeGraph",
     "Engine",
     "KVPool",
+    "PagePool",
+    "PagedDecoder",
     "PoolFull",
     "QWEN3_0_6B",
     "Qwen3Config",
