@@ -359,7 +359,7 @@ int rib_paged_evict(const rib_paged_cache *cache, const int32_t *new_table, long
   s.new_width = new_score_rows;
   // CTAs of a cluster: more while they fit one wave and each still has 4096 rows
   int ctas = 1;
-  while (ctas < 8 && 2LL * ctas * batch * cache->nkv <= 2 * sm_count() && max_len >= 8192 * ctas) ctas *= 2;
+  while (ctas < 8 && 2LL * ctas * batch * cache->nkv <= sm_count() && max_len >= 8192 * ctas) ctas *= 2;
   const int part = ceil_div(max_len, ctas * kSelThreads) * kSelThreads;
   const bool fits = part <= kSelMostRows;
   const auto select = fits ? select_rows_kernel<true> : select_rows_kernel<false>;

@@ -29,13 +29,17 @@ struct SelectParams {
 
 // A score as an unsigned number of the same order; NaN lowest, -0 equal to +0.
 __device__ __forceinline__ uint32_t order_key(float x) {
-  if (x != x) return 0u;
-  const uint32_t u = __float_as_uint(x + 0.0f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const int u = __float_as_int(x + 0.0f);
+  return x == x ? static_cast<uint32_t>(u ^ ((u >> 31) | 0x80000000)) : 0u;
 }
 
-constexpr int kSelMostRows = 24576;  // rows that a CTA keeps in shared memory (two CTAs to an SM)
+constexpr int kSelMostRows = 32768;  // rows that a CTA keeps in shared memory
 static_assert(kSelMostRows <= 32 * kSelThreads, "a lane for each 32 rows of a warp's run");
+
+// The score that a key stands for (a NaN for NaN, +0 for -0).
+__device__ __forceinline__ float score_of(uint32_t key) {
+  return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
 
 // One cluster per (KV head, sequence); CTA r of it takes the r-th part of the rows, a warp a
 // consecutive run of the part, 32 at a time, so the kept rows come out in order.
@@ -46,12 +50,13 @@ static_assert(kSelMostRows <= 32 * kSelThreads, "a lane for each 32 rows of a wa
 // holds the wanted rank.  The walk ends early when all of that bin stays, mostly after two of the three
 // digits.  The first digit is the sign, the exponent and two more bits: accumulated weights have few
 // exponents, and with 8 bits a digit their additions queue at a handful of bins.
-// kCached: the scores are read once, into shared memory; longer parts are read again for every digit.
+// kCached: the scores are read once and kept as keys in shared memory; longer parts are read again for
+// every digit.  What bounds it then is the instructions a row takes in the passes over the keys.
 template <bool kCached>
 __global__ void __launch_bounds__(kSelThreads, 2) select_rows_kernel(const __grid_constant__ SelectParams p) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
-  extern __shared__ float cached[];
+  extern __shared__ __align__(16) uint32_t cached[];
   __shared__ uint32_t hist[2][kSelBins];  // own counts, the cluster's
   __shared__ uint32_t warp_sum[kSelWarps];
   __shared__ int n_gt[kSelWarps], n_eq[kSelWarps];
@@ -81,11 +86,23 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_rows_kernel(const __gri
   const int base = min(rank_in * part, n), mine = min(part, n - base);
   const float *from = sc + base;
   if (kCached) {
-    for (int i = tid; i < mine; i += kSelThreads)
+    const int four = (reinterpret_cast<uintptr_t>(from) & 15u) ? 0 : mine / 4;  // rows by 16 bytes where aligned
+    for (int i = tid; i < four; i += kSelThreads)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(cached + 4 * i)), "l"(from + 4 * i)
+                   : "memory");
+    for (int i = 4 * four + tid; i < mine; i += kSelThreads)
       asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(cached + i)), "l"(from + i) : "memory");
     asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
-    from = cached;
+    // a thread turns the scores that it copied itself into keys
+    for (int i = tid; i < four; i += kSelThreads) {
+      uint4 x = reinterpret_cast<uint4 *>(cached)[i];
+      x = make_uint4(order_key(__uint_as_float(x.x)), order_key(__uint_as_float(x.y)),
+                     order_key(__uint_as_float(x.z)), order_key(__uint_as_float(x.w)));
+      reinterpret_cast<uint4 *>(cached)[i] = x;
+    }
+    for (int i = 4 * four + tid; i < mine; i += kSelThreads) cached[i] = order_key(__uint_as_float(cached[i]));
   }
+  auto key_at = [&](int i) { return kCached ? cached[i] : order_key(from[i]); };
   for (int i = tid; i < kSelBins; i += kSelThreads) hist[0][i] = 0;
   __syncthreads();
   const int lo = p.sinks - base, hi = n - p.recent - base;      // candidates [lo, hi) of the part
@@ -96,8 +113,9 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_rows_kernel(const __gri
     for (int digit = 0; digit < 3; ++digit) {
       const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
       const uint32_t bits = digit == 2 ? 1023u : 2047u;
+#pragma unroll 4
       for (int i = max(lo, 0) + tid; i < min(hi, mine); i += kSelThreads) {
-        const uint32_t key = order_key(from[i]);
+        const uint32_t key = key_at(i);
         if ((key & known) == prefix) atomicAdd(&hist[0][(key >> shift) & bits], 1u);
       }
       const uint32_t *total = hist[0];
@@ -143,25 +161,57 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_rows_kernel(const __gri
   const int ties = static_cast<int>(rank);
   // ---- ordered write: class 2 stays for certain, class 1 matches the threshold
   const int w_lo = warp * per * 32;
-  auto cls = [&](int i) {
-    if (i >= mine) return 0;
-    if (i < lo || i >= hi) return 2;
-    if (stay == 0) return 0;
-    const uint32_t key = order_key(from[i]) & known;
-    return key > prefix ? 2 : key == prefix ? 1 : 0;
-  };
-  // lane v keeps the classes of the run's v-th 32 rows (with 32 of those at most)
-  uint32_t kept_gt = 0, kept_eq = 0;
-  int gt = 0, eq = 0;
-  for (int v = 0; v < per; ++v) {
-    const int k = cls(w_lo + v * 32 + lane);
-    const uint32_t mg = __ballot_sync(0xffffffffu, k == 2), me = __ballot_sync(0xffffffffu, k == 1);
-    gt += __popc(mg);
-    eq += __popc(me);
-    if (kCached && lane == v) {
-      kept_gt = mg;
-      kept_eq = me;
+  const int in_lo = max(lo, 0), in_hi = stay ? min(hi, mine) : 0;  // rows that go by their keys
+  // the classes of rows i0 .. i0 + 31 as masks
+  auto classes = [&](int i0, uint32_t &mg, uint32_t &me) {
+    if (i0 >= in_lo && i0 + 32 <= in_hi) {  // the same for the whole warp
+      const uint32_t key = key_at(i0 + lane) & known;
+      mg = __ballot_sync(0xffffffffu, key > prefix);
+      me = __ballot_sync(0xffffffffu, key == prefix);
+    } else {
+      const int i = i0 + lane;
+      const bool by_key = i >= in_lo && i < in_hi;
+      const uint32_t key = by_key ? key_at(i) & known : 0;
+      mg = __ballot_sync(0xffffffffu, by_key ? key > prefix : i < mine && (i < lo || i >= hi));
+      me = __ballot_sync(0xffffffffu, by_key && key == prefix);
     }
+  };
+  // Cached: lane v keeps the classes of the run's v-th 32 rows (there are 32 of those at most), and how
+  // many rows of each class come before them in the run.
+  uint32_t kept_gt = 0, kept_eq = 0;
+  int gt = 0, eq = 0, before_gt = 0, before_eq = 0;
+#pragma unroll 4
+  for (int v = 0; v < per; ++v) {
+    uint32_t mg, me;
+    classes(w_lo + v * 32, mg, me);
+    if (kCached) {
+      if (lane == v) {
+        kept_gt = mg;
+        kept_eq = me;
+      }
+    } else {
+      gt += __popc(mg);
+      eq += __popc(me);
+    }
+  }
+  if (kCached) {
+    gt = __popc(kept_gt);
+    eq = __popc(kept_eq);
+    before_gt = gt;
+    before_eq = eq;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int ug = __shfl_up_sync(0xffffffffu, before_gt, o), ue = __shfl_up_sync(0xffffffffu, before_eq, o);
+      if (lane >= o) {
+        before_gt += ug;
+        before_eq += ue;
+      }
+    }
+    const int all_gt = __shfl_sync(0xffffffffu, before_gt, 31), all_eq = __shfl_sync(0xffffffffu, before_eq, 31);
+    before_gt -= gt;
+    before_eq -= eq;
+    gt = all_gt;
+    eq = all_eq;
   }
   if (lane == 0) {
     n_gt[warp] = gt;
@@ -185,22 +235,24 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_rows_kernel(const __gri
   for (int v = 0; v < per; ++v) {
     const int i = w_lo + v * 32 + lane;
     uint32_t mg, me;
+    int g = g0, e = e0;
     if (kCached) {
       mg = __shfl_sync(0xffffffffu, kept_gt, v);
       me = __shfl_sync(0xffffffffu, kept_eq, v);
+      g += __shfl_sync(0xffffffffu, before_gt, v);
+      e += __shfl_sync(0xffffffffu, before_eq, v);
     } else {
-      const int k = cls(i);
-      mg = __ballot_sync(0xffffffffu, k == 2);
-      me = __ballot_sync(0xffffffffu, k == 1);
+      classes(w_lo + v * 32, mg, me);
+      g0 += __popc(mg);
+      e0 += __popc(me);
     }
-    const int e = e0 + __popc(me & below);
+    if (!(mg | me)) continue;
+    if (me) e += __popc(me & below);
     if ((mg & bit) || ((me & bit) && e < ties)) {
-      const int at = g0 + __popc(mg & below) + min(e, ties);
+      const int at = g + __popc(mg & below) + min(e, ties);
       rows[at] = base + i;
-      if (ns) ns[at] = from[i];
+      if (ns) ns[at] = kCached ? score_of(cached[i]) : from[i];
     }
-    g0 += __popc(mg);
-    e0 += __popc(me);
   }
   if (ns)
     for (int i = p.keep + rank_in * kSelThreads + tid; i < p.new_width; i += ctas * kSelThreads) ns[i] = 0.f;
