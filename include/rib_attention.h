@@ -645,9 +645,12 @@ int rib_tp_reduce_add_rms(const rib_tp_prefill_exchange *ex, int M,
  * 8; the last dimension is contiguous).  Row r of sequence s lies in page
  * table[s][r / page_rows] at r % page_rows.  A table entry outside
  * [0, num_pages) names no page; entries behind a sequence's rows are never
- * read.  None of the calls keeps state or needs a cleared workspace, so calls
- * on different streams, and captured graphs, are independent as long as each
- * has buffers of its own.
+ * read.  width * page_rows is at most 0x7f000000.  None of the calls keeps
+ * state or needs a cleared workspace, so calls on different streams, and
+ * captured graphs, are independent as long as each has buffers of its own.
+ * Like this library's other kernels they trigger programmatic launch, so
+ * their results are not among the rows that rib_decode_attention_qkv may read
+ * when it is the very next launch.
  *   pages   [num_pages][2][nkv][page_rows][head_dim], K then V
  *   table   [seqs][width] int32, `table_stride` entries from row to row
  * ------------------------------------------------------------------------ */
@@ -700,7 +703,9 @@ int rib_paged_append(const rib_paged_cache *cache, const rib_rotary *rot,
  *   q [batch][nq][head_dim] (strides q_seq, q_head), out the same, contiguous;
  *   nq a multiple of nkv; head_dim 64 or 128; page_rows a multiple of 16;
  *   max_len >= every lens[b], at most width * page_rows.
- * lens[b] == 0 gives a row of zeros.  With `scores` and `scores_out` (FP32
+ * lens[b] == 0 gives a row of zeros.  What pages hold behind a sequence's rows
+ * (infinities, NaN) has no effect; an infinite V value within them gives NaN.
+ * With `scores` and `scores_out` (FP32
  * [batch][nkv][>= max_len], rows contiguous; they may be the same buffer):
  *   scores_out[b][h][n] = scores[b][h][n] + the softmax weight of row n
  * summed over the query heads of KV head h, for n < lens[b]; entries behind
@@ -726,10 +731,12 @@ int rib_paged_decode_attention(const rib_paged_cache *cache, const void *q,
  * the keep - sinks - recent rows with the highest scores (equal scores: the
  * lower row; NaN lowest); shorter sequences keep all.  The kept rows of K and
  * V move, in order, to rows 0, 1, ... of new_table's pages (pages of the same
- * tensor that the old table does not name), their scores to new_scores
+ * tensor that the old table does not name; the table has to hold
+ * min(keep, max_len) rows), their scores to new_scores
  * [batch][nkv][new_score_rows] (or NULL; zeros behind them; not overlapping
  * scores).  rows [batch][nkv][keep] receives the old row numbers, -1 behind
- * them, new_lens [batch] the new lengths.  head_dim 64 or 128. */
+ * them, new_lens [batch] the new lengths.  head_dim 64 or 128; batch and nkv
+ * at most 65535. */
 int rib_paged_evict(const rib_paged_cache *cache, const int32_t *new_table,
                     long long new_table_stride, int new_width,
                     const int32_t *lens, int batch, int max_len,

@@ -22,7 +22,7 @@ int paged_view(const rib_paged_cache *c, rib::paged::View *v) {
       c->head_dim > 256 || c->head_dim % 16 || c->table_stride < 0 || c->stride_page < 0 || c->stride_half < 0 ||
       c->stride_head < 0 || c->stride_row < c->head_dim)
     return RIB_EINVAL;
-  if (static_cast<long long>(c->width) * c->page_rows > 0x7fffffffLL) return RIB_EINVAL;  // rows are 32-bit numbers
+  if (static_cast<long long>(c->width) * c->page_rows > 0x7f000000LL) return RIB_EINVAL;  // rows are 32-bit numbers
   if (!aligned16(c->pages) || !aligned4(c->table) ||
       !strides8(c->stride_page, c->stride_half, c->stride_head, c->stride_row))
     return RIB_EALIGN;
@@ -131,8 +131,12 @@ bool paged_map(CUtensorMap *m, const rib_paged_cache *c) {
   if (!enc) return false;
   cuuint64_t dims[5] = {static_cast<cuuint64_t>(c->head_dim), static_cast<cuuint64_t>(c->page_rows),
                         static_cast<cuuint64_t>(c->nkv), 2, static_cast<cuuint64_t>(c->num_pages)};
-  cuuint64_t strides[4] = {static_cast<cuuint64_t>(c->stride_row) * 2, static_cast<cuuint64_t>(c->stride_head) * 2,
-                           static_cast<cuuint64_t>(c->stride_half) * 2, static_cast<cuuint64_t>(c->stride_page) * 2};
+  // the stride of a dimension of one element is never used, but has to be a valid one
+  const auto bytes = [&](long long stride, cuuint64_t size) {
+    return static_cast<cuuint64_t>(size > 1 ? stride : c->stride_row) * 2;
+  };
+  cuuint64_t strides[4] = {bytes(c->stride_row, 2), bytes(c->stride_head, dims[2]), bytes(c->stride_half, 2),
+                           bytes(c->stride_page, dims[4])};
   cuuint32_t box[5] = {64, static_cast<cuuint32_t>(rib::paged::TK), 1, 2, 1};
   cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   const CUresult r =
@@ -154,7 +158,7 @@ int paged_decode_launch(const rib::paged::DecodeParams &p, int grid, cudaStream_
   if (!set_smem_once(kernel, smem, g_paged_smem_done[std::is_same<T, F16>::value][D == 128][kLogits]))
     return rib::host_fail(RIB_ECUDA, "cudaFuncSetAttribute(paged decode smem)", smem);
   const int s = launch_pdl("paged_decode_kernel launch", kernel, dim3(grid), dim3(NT), smem, st, p);
-  if (s != RIB_OK) return s;
+  if (s != RIB_OK || (p.whole && !kLogits)) return s;
   // blocks of row weights: enough to fill the GPU once, of 1024 rows at least
   const long long heads = static_cast<long long>(p.cache.nkv) * p.batch, room = 4LL * sm_count();
   int row_blocks = 0, rows = 0;
@@ -297,6 +301,7 @@ int rib_paged_decode_attention(const rib_paged_cache *cache, const void *q, long
   p.units_per_kv = ceil_div(p.group, HU);
   p.max_len = max_len;
   p.scale2 = static_cast<float>(scale * 1.4426950408889634);
+  p.whole = max_len <= kWholeRows;
   p.part_o = reinterpret_cast<float *>(ws);
   p.part_ml = reinterpret_cast<float *>(ws + l.ml_off);
   p.rec = reinterpret_cast<JoinRecord *>(ws + l.rec_off);
@@ -334,7 +339,7 @@ int rib_paged_evict(const rib_paged_cache *cache, const int32_t *new_table, long
   if (!lens || !scores || !rows || !new_lens || batch < 1 || batch > cache->seqs || batch > 65535 ||
       cache->nkv > 65535 || max_len < 1 || max_len > static_cast<long long>(cache->width) * cache->page_rows ||
       keep < 1 || sinks < 0 || recent < 0 || static_cast<long long>(sinks) + recent > keep ||
-      keep > static_cast<long long>(new_width) * cache->page_rows || (new_scores && new_score_rows < keep) ||
+      std::min(keep, max_len) > static_cast<long long>(new_width) * cache->page_rows || (new_scores && new_score_rows < keep) ||
       (cache->head_dim != 64 && cache->head_dim != 128))
     return RIB_EINVAL;
   if (!aligned4(lens) || !aligned4(scores) || !aligned4(rows) || !aligned4(new_lens) || !aligned4(new_scores))
@@ -372,7 +377,7 @@ int rib_paged_evict(const rib_paged_cache *cache, const int32_t *new_table, long
   m.rows = rows;
   m.keep = keep;
   return launch_pdl("move_rows_kernel launch", cache->head_dim == 128 ? move_rows_kernel<128> : move_rows_kernel<64>,
-                    dim3(ceil_div(keep, kMoveThreads / 32 * kMoveRows), cache->nkv, batch), dim3(kMoveThreads), 0, st, m);
+                    dim3(ceil_div(std::min(keep, max_len), kMoveThreads / 32 * kMoveRows), cache->nkv, batch), dim3(kMoveThreads), 0, st, m);
 }
 
 }  // extern "C"

@@ -13,6 +13,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -69,6 +70,9 @@ const at::Tensor &tensor(PyObject *o, const char *name, int dim, at::ScalarType 
   return t;
 }
 
+// A stride as the C ABI takes it: that of a dimension of one element is never used.
+int64_t step(const at::Tensor &t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+
 // A tensor that a kernel writes: no two of its elements may share memory by a stride of 0.
 const at::Tensor &written(const at::Tensor &t, const char *name) {
   for (int64_t i = 0; i < t.dim(); ++i)
@@ -119,11 +123,11 @@ rib_paged_cache cache_of(PyObject *pages_o, PyObject *table_o, const at::Tensor 
   if (table.numel() == 0) refuse("table must be [sequences, width], got %s", shape_of(table).c_str());
   c.pages = pages.data_ptr();
   c.table = table.const_data_ptr<int32_t>();
-  c.table_stride = table.stride(0);
-  c.stride_page = pages.stride(0);
+  c.table_stride = step(table, 0);
+  c.stride_page = step(pages, 0);
   c.stride_half = pages.stride(1);
-  c.stride_head = pages.stride(2);
-  c.stride_row = pages.stride(3);
+  c.stride_head = step(pages, 2);
+  c.stride_row = pages.size(3) > 1 ? pages.stride(3) : pages.size(4);
   c.num_pages = size32(pages.size(0), "pages");
   c.nkv = size32(pages.size(2), "pages");
   c.page_rows = size32(pages.size(3), "pages");
@@ -206,8 +210,8 @@ PyObject *rotary(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const c10::cuda::CUDAGuard guard(dev);
     const at::Tensor out = output(a[3], x, "out");
     if (x.numel() > 0)
-      checked(rotary_apply(&rot, x.const_data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0),
-                           out.stride(1), pos, tokens, nh, static_cast<int>(x.size(2)), dtype, stream_of(dev)),
+      checked(rotary_apply(&rot, x.const_data_ptr(), step(x, 0), step(x, 1), out.data_ptr(), step(out, 0),
+                           step(out, 1), pos, tokens, nh, static_cast<int>(x.size(2)), dtype, stream_of(dev)),
               "rotary");
     return THPVariable_Wrap(out);
   });
@@ -241,9 +245,9 @@ PyObject *paged_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const c10::cuda::CUDAGuard guard(dev);
     const at::Tensor out = output(a[12], q, "out");
     if (tokens > 0)
-      checked(paged_append_fn(&cache, &rot, q.const_data_ptr(), q.stride(0), q.stride(1), k.const_data_ptr(),
-                              k.stride(0), k.stride(1), v.const_data_ptr(), v.stride(0), v.stride(1), out.data_ptr(),
-                              out.stride(0), out.stride(1), pos, row, seq, tokens, nq, w[0], w[1],
+      checked(paged_append_fn(&cache, &rot, q.const_data_ptr(), step(q, 0), step(q, 1), k.const_data_ptr(),
+                              step(k, 0), step(k, 1), v.const_data_ptr(), step(v, 0), step(v, 1), out.data_ptr(),
+                              step(out, 0), step(out, 1), pos, row, seq, tokens, nq, w[0], w[1],
                               static_cast<float>(eps), stream_of(dev)),
               "paged_append");
     return THPVariable_Wrap(out);
@@ -305,7 +309,7 @@ PyObject *paged_decode_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
       const at::Tensor &t = a[7] == Py_None ? s : scores_of(a[7], "scores_out", batch, cache.nkv, max_len, dev);
       in = s.const_data_ptr<float>();
       to = written(t, "scores_out").data_ptr<float>();
-      in_s[0] = s.stride(0), in_s[1] = s.stride(1), to_s[0] = t.stride(0), to_s[1] = t.stride(1);
+      in_s[0] = step(s, 0), in_s[1] = step(s, 1), to_s[0] = step(t, 0), to_s[1] = step(t, 1);
       const auto x = span(s), y = span(t);
       if (x.first < y.second && y.first < x.second && (in != to || in_s[0] != to_s[0] || in_s[1] != to_s[1]))
         refuse("scores_out must be scores itself or not overlap it");
@@ -318,7 +322,7 @@ PyObject *paged_decode_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const size_t bytes = decode_workspace_bytes(batch, max_len, nq, cache.head_dim, in != nullptr);
     // scratch of this call alone: the allocator hands it on in stream order
     const at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, pages->options().dtype(at::kByte));
-    checked(decode_attention_fn(&cache, q.const_data_ptr(), q.stride(0), q.stride(1), lens, batch, nq, max_len,
+    checked(decode_attention_fn(&cache, q.const_data_ptr(), step(q, 0), step(q, 1), lens, batch, nq, max_len,
                                 static_cast<float>(scale), out.data_ptr(), in, in_s[0], in_s[1], to, to_s[0], to_s[1],
                                 ws.data_ptr(), bytes, stream_of(dev)),
             "paged_decode_attention");
@@ -342,8 +346,9 @@ PyObject *paged_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const int keep = number(a[4], "keep"), sinks = number(a[6], "sinks"), recent = number(a[7], "recent");
     if (keep < 1 || sinks < 0 || recent < 0 || static_cast<int64_t>(sinks) + recent > keep)
       refuse("need keep >= 1, sinks >= 0, recent >= 0 and sinks + recent <= keep");
-    if (table.size(0) < batch || table.size(1) * cache.page_rows < keep)
-      refuse("new_table must name pages for %d rows of %d sequences, got %s", keep, batch, shape_of(table).c_str());
+    const int most = std::min(keep, max_len);
+    if (table.size(0) < batch || table.size(1) * cache.page_rows < most)
+      refuse("new_table must name pages for %d rows of %d sequences, got %s", most, batch, shape_of(table).c_str());
     float *kept = nullptr;
     int64_t kept_s[2] = {0, 0};
     int kept_rows = 0;
@@ -352,15 +357,15 @@ PyObject *paged_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
       const auto x = span(scores), y = span(t);
       if (x.first < y.second && y.first < x.second) refuse("new_scores must not overlap scores");
       kept = written(t, "new_scores").data_ptr<float>();
-      kept_s[0] = t.stride(0), kept_s[1] = t.stride(1);
+      kept_s[0] = step(t, 0), kept_s[1] = step(t, 1);
       kept_rows = size32(t.size(2), "new_scores");
     }
     const c10::cuda::CUDAGuard guard(dev);
     const auto ints = pages->options().dtype(at::kInt);
     const at::Tensor rows = at::empty({batch, cache.nkv, keep}, ints), new_lens = at::empty({batch}, ints);
-    checked(paged_evict_fn(&cache, table.const_data_ptr<int32_t>(), table.stride(0),
+    checked(paged_evict_fn(&cache, table.const_data_ptr<int32_t>(), step(table, 0),
                            size32(table.size(1), "new_table"), lens, batch, max_len, scores.const_data_ptr<float>(),
-                           scores.stride(0), scores.stride(1), keep, sinks, recent, rows.data_ptr<int32_t>(),
+                           step(scores, 0), step(scores, 1), keep, sinks, recent, rows.data_ptr<int32_t>(),
                            new_lens.data_ptr<int32_t>(), kept, kept_s[0], kept_s[1], kept_rows, stream_of(dev)),
             "paged_evict");
     PyObject *pair = PyTuple_New(2);

@@ -10,7 +10,8 @@
 // lengths on the device: ragged batches and single long sequences fill the GPU alike, and the host
 // never needs the lengths.  A CTA writes the units that lie wholly in its run, and one partial
 // (m, l, o) for the unit its run begins within and one for the unit it ends within; join_kernel sums
-// those in run order.  Nothing in the workspace has to be cleared, and no order depends on timing.
+// those in run order.  (Few tiles: pieces of units instead of runs; short units: whole, with no join.)
+// Nothing in the workspace has to be cleared, and no order depends on timing.
 //
 // In a CTA each of NW warps takes every NW-th tile and feeds itself: lane 0 copies its next tiles into
 // a ring of ST slots of the warp's own by TMA (one 5-D box per 64 dims: 16 rows of K and of V of one
@@ -34,7 +35,11 @@ constexpr int TK = 16;        // rows of a tile: one TMA box, one page at most
 constexpr int NW = 4;         // warps of a CTA
 constexpr int NT = NW * 32;
 constexpr int HU = 8;         // query heads of a unit
-constexpr int kMinTiles = 8;  // fewest tiles of a CTA's run while other CTAs idle
+constexpr int kMinTiles = 8;  // tiles of a piece where CTAs idle: two for each warp
+// Where no sequence can have more rows than this, units stay whole and nothing is launched to join them
+// (8 x 256 rows: 7.3 us, split and joined 8.4; 64 x 100-200 rows: 13.9, 17.4.  With 512 rows it depends
+// on the batch: 64 sequences 25.4 whole, 28.6 split, 8 sequences 11.0 and 9.2).
+constexpr int kWholeRows = 256;
 
 template <int D>
 struct DecodeCfg {
@@ -51,8 +56,8 @@ struct DecodeSmem {
   alignas(16) float o[NW][NW - 1][HU][D / NW + 8];
   float m[NW][HU], l[NW][HU];
   uint64_t full[NW][DecodeCfg<D>::ST];
-  long long sum[NW];                              // tiles of each warp's sequences
-  long long start_tiles;                          // tiles before the run's first sequence
+  long long sum[2][NW];                           // tiles or pieces of each warp's sequences
+  long long start_piece;                          // pieces before the run's first sequence
   int start_seq, start_rows;                      // that sequence and its rows
 };
 
@@ -81,6 +86,7 @@ struct DecodeParams {
   float *scores_out;
   long long in_seq, in_head, out_seq, out_head;
   long long logit_row;          // max_len rounded up to whole tiles
+  int whole;                    // no unit is split over CTAs, and nothing is left to join
 };
 
 __device__ __forceinline__ void tma_load_5d(void *dst, const void *tmap, int c0, int c1, int c2, int c3, int c4,
@@ -171,49 +177,68 @@ __global__ void __launch_bounds__(NT, DecodeCfg<D>::CTAS) paged_decode_kernel(co
   pdl_launch_dependents();
   pdl_wait();
 
-  // ---- this CTA's run of the line: every thread sums the tiles of a block of sequences
+  // ---- this CTA's run of the line.  Every thread sums a block of sequences: their tiles, and their
+  // pieces of kMinTiles tiles.
   const int per = (p.batch + NT - 1) / NT;
   const int b_lo = min(tid * per, p.batch), b_hi = min(b_lo + per, p.batch);
-  long long mine = 0;
   int first_rows = 0;
+  long long mine = 0, mine_short = 0;
   for (int b = b_lo; b < b_hi; ++b) {
-    const int n = seq_rows(p, b);
+    const int n = seq_rows(p, b), t = (n + TK - 1) / TK;
     if (b == b_lo) first_rows = n;
-    mine += (n + TK - 1) / TK;
+    mine += t;
+    mine_short += (t + kMinTiles - 1) / kMinTiles;
     if (blockIdx.x == 0 && n != p.lens[b]) atomicExch(&g_device_status, RIB_ECAPACITY);
   }
-  long long inc = mine;
+  auto scan_warp = [&](long long v, long long *sum) {  // sum over the warp's lanes up to this one
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += up;
-  }
-  if (lane == 31) sm.sum[warp] = inc;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += up;
+    }
+    if (lane == 31) sum[warp] = v;
+    return v;
+  };
+  auto scan_cta = [&](long long &v, const long long *sum) {  // adds the warps before; returns the total
+    long long total = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      if (w < warp) v += sum[w];
+      total += sum[w];
+    }
+    return total;
+  };
+  long long before = scan_warp(mine, sm.sum[0]) - mine, before_short = scan_warp(mine_short, sm.sum[1]) - mine_short;
   __syncthreads();
-  long long before = inc - mine, all = 0;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    if (w < warp) before += sm.sum[w];
-    all += sm.sum[w];
+  long long all = scan_cta(before, sm.sum[0]) * units;
+  const long long all_short = scan_cta(before_short, sm.sum[1]) * units;
+  // Few tiles: pieces of kMinTiles tiles, one to a CTA, each within one unit, so nothing but the join
+  // is left behind it (1 x 513 rows, 8 KV heads: 7.3 us, in equal runs that cross units 8.6).  Otherwise
+  // (quantum 1) equal runs of tiles, which may begin and end within a unit: pieces would leave CTAs idle.
+  int quantum = 1;
+  if (!p.whole && all_short <= gridDim.x) {
+    quantum = kMinTiles;
+    mine = mine_short;
+    before = before_short;
+    all = all_short;
   }
-  all *= units;
-  // Few tiles: fewer CTAs, each with kMinTiles at least.  CTA i takes `quot` tiles, the first `rest` one more.
-  const int cta = blockIdx.x;
-  const int grid = all < static_cast<long long>(gridDim.x) * kMinTiles
-                       ? (static_cast<int>(all) + kMinTiles - 1) / kMinTiles : gridDim.x;
+  // CTA i takes `quot` pieces, the first `rest` one more.
+  const int cta = blockIdx.x, grid = static_cast<int>(min(static_cast<long long>(gridDim.x), all));
   const long long quot = !grid ? 0 : all >> 31 ? all / grid : static_cast<int>(all) / grid;
   const int rest = static_cast<int>(all - quot * grid);
   const long long s0 = cta * quot + min(cta, rest);
-  const int run = cta < grid ? static_cast<int>(quot + (cta < rest)) : 0;
+  int run = cta < grid ? static_cast<int>(quot + (cta < rest)) : 0;
   if (run && before * units <= s0 && s0 < (before + mine) * units) {
     int b = b_lo, n = first_rows;
-    while (s0 >= (before + (n + TK - 1) / TK) * units) {
-      before += (n + TK - 1) / TK;
+    while (true) {
+      const int t = ((n + TK - 1) / TK + quantum - 1) / quantum;
+      if (s0 < (before + t) * units) break;
+      before += t;
       n = seq_rows(p, ++b);
     }
     sm.start_seq = b;
     sm.start_rows = n;
-    sm.start_tiles = before * units;
+    sm.start_piece = before * units;
   }
   __syncthreads();
   if (!run && tid == 0) p.rec[cta].last = -1;
@@ -228,10 +253,34 @@ __global__ void __launch_bounds__(NT, DecodeCfg<D>::CTAS) paged_decode_kernel(co
   c.b = sm.start_seq;
   c.n = sm.start_rows;
   c.tiles = (c.n + TK - 1) / TK;
+  int last_cta = -1;  // with pieces: the CTA that has the last one of this one's unit
   {
-    const long long in_seq = s0 - sm.start_tiles;
-    c.hu = in_seq >> 31 ? static_cast<int>(in_seq / c.tiles) : static_cast<int>(in_seq) / c.tiles;
-    c.tile = static_cast<int>(in_seq - static_cast<long long>(c.hu) * c.tiles);
+    const long long in_seq = s0 - sm.start_piece;
+    const int k = (c.tiles + quantum - 1) / quantum;  // pieces of the unit
+    c.hu = in_seq >> 31 ? static_cast<int>(in_seq / k) : static_cast<int>(in_seq) / k;
+    c.tile = static_cast<int>(in_seq - static_cast<long long>(c.hu) * k);
+    if (quantum > 1) {  // piece c.tile of k nearly equal ones
+      const int piece = c.tile, q = c.tiles / k, r = c.tiles % k;
+      c.tile = piece * q + min(piece, r);
+      run = q + (piece < r);
+      last_cta = cta - piece + k - 1;
+    }
+  }
+  if (p.whole) {  // short units are not split: the run takes those that begin in it, to their end
+    int f = 0;
+    if (c.tile > 0) {
+      f = c.tiles - c.tile;
+      if (f >= run || !next_unit(p, c, units)) {
+        if (tid == 0) p.rec[cta].last = -1;
+        return;
+      }
+    }
+    int end = f;
+    Place w = c;
+    do {
+      end += w.tiles;
+    } while (end < run && next_unit(p, w, units));
+    run = end - f;
   }
 
   // ---- producer side of the warp: tile i of the warp is the run's tile warp + i * NW
@@ -444,7 +493,7 @@ __global__ void __launch_bounds__(NT, DecodeCfg<D>::CTAS) paged_decode_kernel(co
         int last = -1;  // the CTA in which a unit that begins here and does not end here ends
         if (c.tile == 0 && !whole) {
           const long long x = s0 + f + c.tiles - 1, big = rest * (quot + 1);  // its last tile
-          last = static_cast<int>(x < big ? x / (quot + 1) : rest + (x - big) / quot);
+          last = quantum > 1 ? last_cta : static_cast<int>(x < big ? x / (quot + 1) : rest + (x - big) / quot);
         }
         if (f + seg == run) p.rec[cta] = {c.b, c.hu, last};
         if (kLogits && c.tile == 0) p.span[static_cast<size_t>(c.b) * units + c.hu] = make_int2(cta, last);

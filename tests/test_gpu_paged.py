@@ -245,6 +245,21 @@ def test_attention_sharp_and_large_scores(rib, lib, dtype):
     check_attention(rib, lib, [1000, 77], nq=4, nkv=2, D=128, page_rows=16, dtype=dtype, q_scale=40.0, scores=True)
 
 
+@pytest.mark.parametrize("B,high", [(1, 256), (40, 17), (700, 40), (1500, 1), (333, 256)])
+@pytest.mark.parametrize("scores", [False, True])
+def test_attention_short_tables(rib, lib, B, high, scores):
+    """Tables of at most 256 rows: units are never split; several units to a CTA, and empty sequences."""
+    lens = [(b * 7919) % (high + 1) for b in range(B)]
+    lens[-1] = high
+    check_attention(rib, lib, lens, nq=4, nkv=2, D=64 if B > 1 else 128, page_rows=16, dtype=BF16, scores=scores)
+
+
+@pytest.mark.parametrize("lens", [[4719], [4720], [4737], [4736, 1], [16 * 148], [300] * 12, [3000, 0, 1, 1700]])
+def test_attention_between_pieces_and_runs(rib, lib, lens):
+    """Few tiles are cut into pieces of units, one to a CTA; more than fill the GPU into equal runs."""
+    check_attention(rib, lib, lens, nq=16, nkv=8, D=128, page_rows=16, dtype=FP16, scores=True)
+
+
 def test_attention_max_len_and_wide_table(rib, lib):
     check_attention(rib, lib, [40, 100], nq=2, nkv=1, D=128, page_rows=16, dtype=BF16, max_len=100, width=50, scores=True)
 
@@ -465,6 +480,81 @@ def test_evict_ties_infinities_and_nan(rib, lib):
     for keep, sinks, recent in [(50, 3, 7), (81, 0, 0), (100, 1, 1), (159, 0, 0)]:
         check_evict(rib, lib, [n] * B, nkv=nkv, D=64, page_rows=16, dtype=BF16, keep=keep, sinks=sinks, recent=recent,
                     scores=s.cuda())
+
+
+def test_evict_keep_beyond_the_table(rib, lib):
+    """keep may exceed what any sequence has: every row moves, and the new table holds just those."""
+    g = gen(3)
+    pages, table = make_cache([40, 16], 2, 64, 16, BF16, g, spare=4, fill=0.0)
+    free = sorted(set(range(pages.shape[0])) - set(table.flatten().tolist()))
+    new = i32([[free[0], free[1], free[2]], [free[3], -1, -1]])
+    scores = torch.rand((2, 2, 48), generator=g).cuda()
+    before = pages.clone()
+    rows, n = rib.paged_evict(pages, table, i32([40, 16]), scores, 1000, new)
+    assert n.tolist() == [40, 16] and lib.take_device_status() == 0
+    assert torch.equal(rows[0, :, :40], torch.arange(40, device="cuda", dtype=torch.int32).expand(2, 40))
+    assert (rows[0, :, 40:] == -1).all() and (rows[1, :, 16:] == -1).all()
+    for b, m in enumerate((40, 16)):
+        at = torch.arange(m, device="cuda")
+        assert torch.equal(pages[new[b, at // 16].long(), :, :, at % 16], before[table[b, at // 16].long(), :, :, at % 16])
+
+
+@pytest.mark.parametrize("make", ["zero_stride", "odd_stride"])
+def test_dimensions_of_one_element_have_no_stride(rib, lib, make):
+    """One page, one KV head, one token: their strides are never used, whatever they are."""
+    g = gen(4)
+    base = torch.randn((1, 2, 1, 16, 64), generator=g).to(BF16).cuda()
+    odd = 0 if make == "zero_stride" else 3
+    pages = base.as_strided(base.shape, (odd, 1024, odd, 64, 1))
+    table = i32([0]).as_strided((1, 1), (odd, 1))
+    q = torch.randn((1, 2, 64), generator=g).to(BF16).cuda()
+    one = q.as_strided((1, 2, 64), (odd, 64, 1))
+    want, _, bound, _ = attend64(q, base, i32([[0]]), [9], 0.125)
+    close(rib.paged_decode_attention(one, pages, table, i32([9]), 0.125), want, bound)
+    rot = rib.Rotary(64)
+    k = q[:, :1]
+    got = rib.paged_append(one, k, k, i32([5]), i32([9]), pages, table, rot)
+    assert torch.equal(got, rib.rotary(q, i32([5]), rot))
+    assert torch.equal(base[0, 1, 0, 9], k[0, 0]) and torch.equal(base[0, 0, 0, 9], rib.rotary(k, i32([5]), rot)[0, 0])
+    assert lib.take_device_status() == 0
+
+
+def test_outputs_that_overlap_are_refused(rib, lib):
+    g = gen(5)
+    pages, table = make_cache([32, 32], 2, 64, 16, BF16, g)
+    q = torch.randn((2, 4, 64), generator=g).to(BF16).cuda()
+    n = i32([32, 32])
+    scores = torch.zeros((2, 2, 64), device="cuda")
+    for kw in (dict(scores=scores[..., :40], scores_out=scores[..., 8:48]),
+               dict(scores=scores, scores_out=scores[:1, :1].expand(2, 2, 64)), dict(scores_out=scores),
+               dict(scores=scores[..., :31]), dict(scores=scores.double()), dict(out=q[:, :2]), dict(max_len=33),
+               dict(max_len=0), dict(out=torch.empty((2, 8, 64), dtype=BF16, device="cuda")[:, ::2])):
+        with pytest.raises(ValueError):
+            rib.paged_decode_attention(q, pages, table, n, 0.125, **kw)
+    with pytest.raises(ValueError):
+        rib.paged_evict(pages, table, n, scores, 16, table, new_scores=scores[..., 32:])
+    with pytest.raises(ValueError):
+        rib.paged_append(q, q[:, :2], q[:, :2], n, n, pages[:1].expand(3, -1, -1, -1, -1), table, rib.Rotary(64))
+    with pytest.raises(ValueError):
+        rib.rotary(q, n, rib.Rotary(64), out=q[:, :1].expand(2, 4, 64))
+    for bad in (q.float(), q[..., :32], q.transpose(1, 2), q[0]):
+        with pytest.raises(ValueError):
+            rib.paged_decode_attention(bad, pages, table, n, 0.125)
+    for bad in (table.long(), table[0], table[:1], table[:, :0], table.cpu()):
+        with pytest.raises(ValueError):
+            rib.paged_decode_attention(q, pages, bad, n, 0.125)
+    for bad in (n.long(), n[:1], n.cpu()):
+        with pytest.raises(ValueError):
+            rib.paged_decode_attention(q, pages, table, bad, 0.125)
+    for bad in (pages.float(), pages[:, :1], pages[..., :32], pages[:, :, :, :8], pages[0]):
+        with pytest.raises(ValueError):
+            rib.paged_decode_attention(q, bad, table, n, 0.125)
+    with pytest.raises(ValueError):  # 16-byte alignment
+        rib.rotary(torch.zeros(129, dtype=BF16, device="cuda")[1:].view(1, 2, 64), i32([0]), rib.Rotary(64))
+    out = rib.paged_decode_attention(q, pages, table, n, 0.125)
+    same = q.clone()
+    assert rib.paged_decode_attention(same, pages, table, n, 0.125, out=same) is same and torch.equal(same, out)
+    assert lib.take_device_status() == 0
 
 
 def test_evict_reports_missing_pages(rib, lib):

@@ -45,7 +45,7 @@ def rot(**kw):
 BAD_CACHES = [(dict(pages=None), EINVAL), (dict(table=None), EINVAL), (dict(dtype=2), EINVAL), (dict(num_pages=0), EINVAL),
               (dict(nkv=0), EINVAL), (dict(page_rows=0), EINVAL), (dict(head_dim=24), EINVAL), (dict(head_dim=72), EINVAL),
               (dict(head_dim=272), EINVAL), (dict(seqs=0), EINVAL), (dict(width=0), EINVAL), (dict(stride_row=32), EINVAL),
-              (dict(stride_page=-8), EINVAL), (dict(width=1 << 28), EINVAL), (dict(pages=MISALIGNED), EALIGN),
+              (dict(stride_page=-8), EINVAL), (dict(width=0x7f0001, page_rows=256), EINVAL), (dict(pages=MISALIGNED), EALIGN),
               (dict(table=FAKE + 2), EALIGN), (dict(stride_row=68), EALIGN), (dict(stride_head=1028), EALIGN)]
 
 
@@ -117,7 +117,7 @@ def test_evict_refuses(rib):
     for kw, status in BAD_CACHES:
         assert call(c=cache(**kw)) == status, kw
     for kw in (dict(table=None), dict(lens=None), dict(scores=None), dict(rows=None), dict(new_lens=None), dict(batch=0),
-               dict(batch=4), dict(max_len=0), dict(max_len=65), dict(keep=0), dict(keep=33), dict(sinks=-1),
+               dict(batch=4), dict(max_len=0), dict(max_len=65), dict(keep=0), dict(keep=33, new_rows=33), dict(sinks=-1),
                dict(recent=-1), dict(sinks=16, recent=17), dict(sinks=2 ** 31 - 1, recent=2 ** 31 - 1), dict(new_rows=31),
                dict(width=0), dict(stride=-1), dict(c=cache(head_dim=96, stride_row=96))):
         assert call(**kw) == EINVAL, kw
