@@ -16,12 +16,17 @@
 // In a CTA each of NW warps takes every NW-th tile and feeds itself: lane 0 copies its next tiles into
 // a ring of ST slots of the warp's own by TMA (one 5-D box per 64 dims: 16 rows of K and of V of one
 // page), so warps never wait for each other within a unit.  Scores and P.V run on mma.m16n8k16 with
-// the heads as the 16 rows.  A decode step reads 2 D bytes per row for 4 D flops per query head, so
-// memory bounds it at any group size here; at 8 heads per KV head the tensor pipe is busy for under a
-// fifth of the time a tile's copy takes, and a tcgen05 tile (128 rows at least, accumulators in TMEM)
-// would add a round trip through TMEM for rows that stay empty.  The upper 8 rows of the A operand are
-// free with 8 heads: in P.V they carry p - round(p), so P enters with 16 (BF16) or 22 (FP16) bits and
-// its rounding adds nothing to the output's.
+// the heads as the 16 rows.  A decode step reads 4 D bytes per row for 4 D flops per query head, so
+// memory bounds it at any group size here (8 heads per KV head: 52 TFLOP/s at the full memory rate), and
+// a tcgen05 tile (128 rows at least, accumulators in TMEM) would add a round trip through TMEM for rows
+// that stay empty.  The upper 8 rows of the A operand are free with 8 heads: in P.V they carry
+// p - round(p), so P enters with 16 (BF16) or 22 (FP16) bits and its rounding adds nothing to the
+// output's.
+//
+// Measured on B200 (one launch pair, state larger than L2): 64 sequences of 30-33k rows, 8 KV heads of
+// 64 dims, 605-633 us (6.5-6.8 TB/s); 32 x 8191 rows, 64 heads over 8, FP16, 165-169 us (6.4-6.5 TB/s,
+// DRAM reads 1.000 of the rows' bytes); 64 x 512-4096 rows with row weights 108-110 us (of them 13 us for
+// join and weights); 1 x 32769 rows 30 us, of which the copies take 20.
 #pragma once
 
 #include <cuda.h>
@@ -43,6 +48,8 @@ constexpr int kWholeRows = 256;
 
 template <int D>
 struct DecodeCfg {
+  // 128 KB (144 KB) of tiles under way on an SM.  More is slower: with 3 slots at D = 128 the 32 x 8191
+  // rows above take 182 us instead of 168, with 4 at D = 64 the large batch 662 instead of 630.
   static constexpr int CTAS = D == 128 ? 2 : 3;   // resident per SM
   static constexpr int ST = D == 128 ? 2 : 3;     // ring slots of a warp
   static constexpr int HALF = 2 * TK * 128;       // bytes of one box: 64 dims of K and of V rows
@@ -285,6 +292,8 @@ __global__ void __launch_bounds__(NT, DecodeCfg<D>::CTAS) paged_decode_kernel(co
 
   // ---- producer side of the warp: tile i of the warp is the run's tile warp + i * NW
   const int count = run > warp ? (run - warp + NW - 1) / NW : 0;
+  // Rows are read once: kept out of L2's way (evict first), a sustained large batch runs at a steady
+  // 620 us; with the default priority it wandered between 607 and 866.  Units that share rows leave them.
   const uint64_t policy = p.units_per_kv == 1 ? l2_policy_evict_first() : l2_policy_evict_normal();
   // moves `by` tiles along the run
   auto seek = [&](Place &pl, int by) {
