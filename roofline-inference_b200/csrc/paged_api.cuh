@@ -98,7 +98,7 @@ int launch_cluster(const char *what, void (*kernel)(KArgs...), dim3 grid, dim3 b
 
 // ------------------------------------------------------------------ paged decode
 struct PagedDecodeLayout {
-  size_t ml_off, rec_off, lse_off, span_off, logits_off, total;
+  size_t ml_off, rec_off, norm_off, span_off, logits_off, total;
   long long logit_row;
   int grid;
 };
@@ -113,9 +113,9 @@ PagedDecodeLayout paged_decode_layout(int batch, int max_len, int nq, int dim, b
   l.rec_off = off;
   off += round256(static_cast<size_t>(l.grid) * sizeof(JoinRecord));
   l.logit_row = (static_cast<long long>(max_len) + TK - 1) / TK * TK;
-  l.lse_off = l.span_off = l.logits_off = off;
+  l.norm_off = l.span_off = l.logits_off = off;
   if (scores) {
-    off += round256(static_cast<size_t>(batch) * nq * sizeof(float));
+    off += round256(static_cast<size_t>(batch) * nq * sizeof(float2));
     l.span_off = off;  // at most one unit a query head
     off += round256(static_cast<size_t>(batch) * nq * sizeof(int2));
     l.logits_off = off;
@@ -307,7 +307,7 @@ int rib_paged_decode_attention(const rib_paged_cache *cache, const void *q, long
   p.rec = reinterpret_cast<JoinRecord *>(ws + l.rec_off);
   p.logit_row = l.logit_row;
   if (scores) {
-    p.lse = reinterpret_cast<float *>(ws + l.lse_off);
+    p.norm = reinterpret_cast<float2 *>(ws + l.norm_off);
     p.span = reinterpret_cast<int2 *>(ws + l.span_off);
     p.logits = reinterpret_cast<float *>(ws + l.logits_off);
     p.scores = scores;

@@ -21,7 +21,8 @@
 // a tcgen05 tile (128 rows at least, accumulators in TMEM) would add a round trip through TMEM for rows
 // that stay empty.  The upper 8 rows of the A operand are free with 8 heads: in P.V they carry
 // p - round(p), so P enters with 16 (BF16) or 22 (FP16) bits and its rounding adds nothing to the
-// output's.
+// output's.  FP16 weights are lifted by 2^14 (as is their sum), out of the type's subnormal range: many
+// small weights behind one large one add up.
 //
 // Measured on B200 (one launch pair, state larger than L2): 64 sequences of 30-33k rows, 8 KV heads of
 // 64 dims, 605-633 us (6.5-6.8 TB/s); 32 x 8191 rows, 64 heads over 8, FP16, 165-169 us (6.4-6.5 TB/s,
@@ -87,7 +88,7 @@ struct DecodeParams {
   float *part_ml;               // [grid][2][HU][2]
   JoinRecord *rec;              // [grid]
   float *logits;                // [B][nq][logit_row] scores in log2 units, or null
-  float *lse;                   // [B][nq] log2 of the sum of units of one CTA, with logits
+  float2 *norm;                 // [B][nq] (maximum, 1 / sum) of units of one CTA, with logits
   int2 *span;                   // [B][units] first and last CTA of a unit that spans several, or -1
   const float *scores;          // row weights: scores_out = scores + weight, strides below
   float *scores_out;
@@ -164,6 +165,13 @@ __device__ __forceinline__ bool next_unit(const DecodeParams &p, Place &c, int u
     if (c.tiles > 0) return true;
   }
   return false;
+}
+
+// (maximum, factor) such that exp2(score - maximum) * factor is a row's weight.
+template <class T>
+__device__ __forceinline__ float2 weight_norm(float M, float L) {
+  if (L == 0.f) return make_float2(0.f, 0.f);  // every score -inf
+  return make_float2(M, static_cast<float>(1 << T::kLift) / L);
 }
 
 template <class T, int D, bool kLogits>
@@ -425,7 +433,7 @@ __global__ void __launch_bounds__(NT, DecodeCfg<D>::CTAS) paged_decode_kernel(co
       }
       float pr[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) pr[e] = fast_exp2(sc[e] - mz);
+      for (int e = 0; e < 4; ++e) pr[e] = fast_exp2(T::kLift ? sc[e] - mz + T::kLift : sc[e] - mz);
       l += (pr[0] + pr[1]) + (pr[2] + pr[3]);
       // A fragments of P: rows 0-7 the rounded weights, rows 8-15 what the rounding left
       const uint32_t a0 = T::pack(pr[0], pr[1]), a2 = T::pack(pr[2], pr[3]);
@@ -496,7 +504,7 @@ __global__ void __launch_bounds__(NT, DecodeCfg<D>::CTAS) paged_decode_kernel(co
         if (!whole)
           *reinterpret_cast<float2 *>(p.part_ml + ((static_cast<size_t>(cta) * 2 + part) * HU + g) * 2) = make_float2(M, L);
         else if (kLogits)
-          p.lse[static_cast<size_t>(c.b) * p.nq + h0 + g] = L == 0.f ? INFINITY : M + log2f(L);
+          p.norm[static_cast<size_t>(c.b) * p.nq + h0 + g] = weight_norm<T>(M, L);
       }
       if (tid == 0) {
         int last = -1;  // the CTA in which a unit that begins here and does not end here ends
@@ -550,6 +558,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
                                                             int row_blocks, int rows) {
   __shared__ float4 acc[kJoinWarps][D / 4];
   __shared__ float head_sum[kJoinWarps];
+  __shared__ float2 head_norm[kJoinWarps];
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -622,14 +631,14 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     const size_t head0 = static_cast<size_t>(b) * p.nq + h * p.group + u * HU;
     if (warp < heads) {
       const int2 span = p.span[static_cast<size_t>(b) * p.cache.nkv * p.units_per_kv + hu];
-      float lse;
+      float2 norm;
       if (span.y < 0) {
-        lse = p.lse[head0 + warp];
+        norm = p.norm[head0 + warp];
       } else {
         const float2 ml = joined_ml(p, span.x, span.y, warp, lane);
-        lse = ml.y == 0.f ? INFINITY : ml.x + log2f(ml.y);
+        norm = weight_norm<T>(ml.x, ml.y);
       }
-      if (lane == 0) head_sum[warp] = lse;
+      if (lane == 0) head_norm[warp] = norm;
     }
     __syncthreads();
     const float *in = u ? out : p.scores + b * p.in_seq + h * p.in_head + k0;
@@ -650,7 +659,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
         float sum = 0.f;
 #pragma unroll
         for (int g = 0; g < HU; ++g)
-          if (g < heads) sum += fast_exp2(x[g][i] - head_sum[g]);
+          if (g < heads) sum = fmaf(fast_exp2(x[g][i] - head_norm[g].x), head_norm[g].y, sum);
         w[i] += sum;
       }
 #pragma unroll

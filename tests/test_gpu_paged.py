@@ -260,6 +260,30 @@ def test_attention_between_pieces_and_runs(rib, lib, lens):
     check_attention(rib, lib, lens, nq=16, nkv=8, D=128, page_rows=16, dtype=FP16, scores=True)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("gap", [12.0, 17.0, 19.0])
+@pytest.mark.parametrize("n", [200, 30000])
+def test_attention_many_small_weights_behind_one_large(rib, lib, n, gap, dtype):
+    """One row takes nearly all the weight and has V = 0, so the output is what all the others (weights
+    of exp(-gap) each, V near 1) add up to: they must not be lost in the type of P."""
+    g = gen(12)
+    D = 64
+    pages, table = make_cache([n], 1, D, 16, dtype, g)
+    at = torch.arange(n, device="cuda")
+    page, slot = table[0, at // 16].long(), at % 16
+    pages[page, 0, 0, slot] = 0
+    pages[page, 1, 0, slot] = (1 + torch.rand((n, D), generator=g).cuda() / 8).to(dtype)
+    pages[page[n // 3], 0, 0, slot[n // 3], 0] = gap
+    pages[page[n // 3], 1, 0, slot[n // 3]] = 0
+    q = torch.zeros((1, 2, D), dtype=dtype, device="cuda")
+    q[:, :, 0] = 8.0
+    scores = torch.zeros((1, 1, table.shape[1] * 16), device="cuda")
+    want, weights, bound, rel = attend64(q, pages, table, [n], 0.125)
+    got = rib.paged_decode_attention(q, pages, table, i32([n]), 0.125, scores=scores)
+    close(got, want, bound)
+    assert ((scores[0, :, :n].double() - weights[0]).abs() <= weights[0] * (rel[0] + 2.0 ** -24)).all()
+
+
 def test_attention_max_len_and_wide_table(rib, lib):
     check_attention(rib, lib, [40, 100], nq=2, nkv=1, D=128, page_rows=16, dtype=BF16, max_len=100, width=50, scores=True)
 
