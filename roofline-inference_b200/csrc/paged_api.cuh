@@ -148,7 +148,7 @@ bool paged_map(CUtensorMap *m, const rib_paged_cache *c) {
 }
 
 bool g_paged_smem_done[2][2][2][kMaxDevices];
-bool g_select_smem_done[kMaxDevices];
+bool g_select_smem_done[2][kMaxDevices];
 
 template <class T, int D, bool kLogits>
 int paged_decode_launch(const rib::paged::DecodeParams &p, int grid, cudaStream_t st) {
@@ -178,6 +178,23 @@ int paged_decode_launch(const rib::paged::DecodeParams &p, int dim, int grid, cu
   if (dim == 128)
     return p.logits ? paged_decode_launch<T, 128, true>(p, grid, st) : paged_decode_launch<T, 128, false>(p, grid, st);
   return p.logits ? paged_decode_launch<T, 64, true>(p, grid, st) : paged_decode_launch<T, 64, false>(p, grid, st);
+}
+
+template <int kThreads>
+int select_launch(const rib::paged::SelectParams &s, long long units, int batch, cudaStream_t st) {
+  using namespace rib::paged;
+  // CTAs of a cluster: more while they fit one wave and each still has 4096 rows
+  int ctas = 1;
+  while (ctas < 8 && 2 * ctas * units <= sm_count() && s.max_len >= 8192 * ctas) ctas *= 2;
+  const int part = ceil_div(s.max_len, ctas * kThreads) * kThreads;
+  constexpr int most = kSelStepRows * kThreads;
+  const bool fits = part <= most;
+  if (!set_smem_once(select_rows_kernel<kThreads, true>, most * static_cast<int>(sizeof(float)),
+                     g_select_smem_done[kThreads == 1024]))
+    return rib::host_fail(RIB_ECUDA, "cudaFuncSetAttribute(select smem)", most);
+  return launch_cluster("select_rows_kernel launch",
+                        fits ? select_rows_kernel<kThreads, true> : select_rows_kernel<kThreads, false>,
+                        dim3(s.nkv * ctas, batch), dim3(kThreads), fits ? part * sizeof(float) : 0, ctas, st, s);
 }
 
 }  // namespace
@@ -362,17 +379,12 @@ int rib_paged_evict(const rib_paged_cache *cache, const int32_t *new_table, long
   s.recent = recent;
   s.max_len = max_len;
   s.new_width = new_score_rows;
-  // CTAs of a cluster: more while they fit one wave and each still has 4096 rows
-  int ctas = 1;
-  while (ctas < 8 && 2LL * ctas * batch * cache->nkv <= sm_count() && max_len >= 8192 * ctas) ctas *= 2;
-  const int part = ceil_div(max_len, ctas * kSelThreads) * kSelThreads;
-  const bool fits = part <= kSelMostRows;
-  const auto select = fits ? select_rows_kernel<true> : select_rows_kernel<false>;
-  constexpr int most = kSelMostRows * static_cast<int>(sizeof(float));
-  if (!set_smem_once(select_rows_kernel<true>, most, g_select_smem_done))
-    return rib::host_fail(RIB_ECUDA, "cudaFuncSetAttribute(select smem)", most);
-  const int e = launch_cluster("select_rows_kernel launch", select, dim3(cache->nkv * ctas, batch), dim3(kSelThreads),
-                               fits ? part * sizeof(float) : 0, ctas, st, s);
+  // CTAs of 512 threads where rows are few, or few for so many heads that the CTAs queue (us for both
+  // kernels, 512 against 1024 threads: 90 x 8 heads of 700 rows 27 and 33, 3 x 4 of 700 7.7 and 9.2,
+  // 90 x 8 of 2000 76 and 81; but 10 x 4 of 2000 16.5 and 14.2, 30 x 8 of 4000 76 and 71)
+  const long long units = static_cast<long long>(batch) * cache->nkv;
+  const bool few = max_len <= 1024 || (max_len <= 2048 && units > 2 * sm_count());
+  const int e = few ? select_launch<512>(s, units, batch, st) : select_launch<1024>(s, units, batch, st);
   if (e != RIB_OK) return e;
   m.rows = rows;
   m.keep = keep;

@@ -14,7 +14,6 @@
 namespace rib {
 namespace paged {
 
-constexpr int kSelThreads = 1024, kSelWarps = kSelThreads / 32;
 constexpr int kSelBins = 2048;
 
 struct SelectParams {
@@ -33,8 +32,7 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   return x == x ? static_cast<uint32_t>(u ^ ((u >> 31) | 0x80000000)) : 0u;
 }
 
-constexpr int kSelMostRows = 32768;  // rows that a CTA keeps in shared memory
-static_assert(kSelMostRows <= 32 * kSelThreads, "a lane for each 32 rows of a warp's run");
+constexpr int kSelStepRows = 32;  // rows of a thread that a CTA keeps in shared memory: a lane for each step
 
 // The score that a key stands for (a NaN for NaN, +0 for -0).
 __device__ __forceinline__ float score_of(uint32_t key) {
@@ -51,16 +49,17 @@ __device__ __forceinline__ float score_of(uint32_t key) {
 // digits.  The first digit is the sign, the exponent and two more bits: accumulated weights have few
 // exponents, and with 8 bits a digit their additions queue at a handful of bins.
 // kCached: the scores are read once and kept as keys in shared memory; longer parts are read again for
-// every digit.  Reading the scores takes a few us at most; the passes over the keys (instructions, and the
-// histogram's additions) bound it: 35 us for 8 x 8 heads of 65536 rows, 19 us for 32 x 8 of 300-8192.
-template <bool kCached>
-__global__ void __launch_bounds__(kSelThreads, 2) select_rows_kernel(const __grid_constant__ SelectParams p) {
+// every digit.  Reading the scores takes a few us at most; the chain of passes over the keys and the
+// barriers between them bound it: 35 us for 8 x 8 heads of 65536 rows, 19 us for 32 x 8 of 300-8192.
+template <int kThreads, bool kCached>
+__global__ void __launch_bounds__(kThreads, 2048 / kThreads) select_rows_kernel(const __grid_constant__ SelectParams p) {
+  constexpr int kWarps = kThreads / 32;
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ __align__(16) uint32_t cached[];
   __shared__ uint32_t hist[2][kSelBins];  // own counts, the cluster's
-  __shared__ uint32_t warp_sum[kSelWarps];
-  __shared__ int n_gt[kSelWarps], n_eq[kSelWarps];
+  __shared__ uint32_t warp_sum[kWarps];
+  __shared__ int n_gt[kWarps], n_eq[kWarps];
   __shared__ int cta_gt, cta_eq;
   __shared__ uint32_t pick_bin, pick_rank, pick_count;
   pdl_launch_dependents();
@@ -77,34 +76,34 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_rows_kernel(const __gri
   int32_t *rows = p.rows + (static_cast<size_t>(b) * p.nkv + h) * p.keep;
   float *ns = p.new_scores ? p.new_scores + b * p.n_seq + h * p.n_head : nullptr;
   if (n <= p.keep) {  // the same for the whole cluster
-    for (int i = rank_in * kSelThreads + tid; i < p.keep; i += ctas * kSelThreads) rows[i] = i < n ? i : -1;
+    for (int i = rank_in * kThreads + tid; i < p.keep; i += ctas * kThreads) rows[i] = i < n ? i : -1;
     if (ns)
-      for (int i = rank_in * kSelThreads + tid; i < p.new_width; i += ctas * kSelThreads) ns[i] = i < n ? sc[i] : 0.f;
+      for (int i = rank_in * kThreads + tid; i < p.new_width; i += ctas * kThreads) ns[i] = i < n ? sc[i] : 0.f;
     return;
   }
   // this CTA's part of the rows, and of it each warp's run of `per` times 32 rows
-  const int per = (n + ctas * kSelThreads - 1) / (ctas * kSelThreads), part = per * kSelThreads;
+  const int per = (n + ctas * kThreads - 1) / (ctas * kThreads), part = per * kThreads;
   const int base = min(rank_in * part, n), mine = min(part, n - base);
   const float *from = sc + base;
   if (kCached) {
     const int four = (reinterpret_cast<uintptr_t>(from) & 15u) ? 0 : mine / 4;  // rows by 16 bytes where aligned
-    for (int i = tid; i < four; i += kSelThreads)
+    for (int i = tid; i < four; i += kThreads)
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(cached + 4 * i)), "l"(from + 4 * i)
                    : "memory");
-    for (int i = 4 * four + tid; i < mine; i += kSelThreads)
+    for (int i = 4 * four + tid; i < mine; i += kThreads)
       asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(cached + i)), "l"(from + i) : "memory");
     asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
     // a thread turns the scores that it copied itself into keys
-    for (int i = tid; i < four; i += kSelThreads) {
+    for (int i = tid; i < four; i += kThreads) {
       uint4 x = reinterpret_cast<uint4 *>(cached)[i];
       x = make_uint4(order_key(__uint_as_float(x.x)), order_key(__uint_as_float(x.y)),
                      order_key(__uint_as_float(x.z)), order_key(__uint_as_float(x.w)));
       reinterpret_cast<uint4 *>(cached)[i] = x;
     }
-    for (int i = 4 * four + tid; i < mine; i += kSelThreads) cached[i] = order_key(__uint_as_float(cached[i]));
+    for (int i = 4 * four + tid; i < mine; i += kThreads) cached[i] = order_key(__uint_as_float(cached[i]));
   }
   auto key_at = [&](int i) { return kCached ? cached[i] : order_key(from[i]); };
-  for (int i = tid; i < kSelBins; i += kSelThreads) hist[0][i] = 0;
+  for (int i = tid; i < kSelBins; i += kThreads) hist[0][i] = 0;
   __syncthreads();
   const int lo = p.sinks - base, hi = n - p.recent - base;      // candidates [lo, hi) of the part
   const uint32_t stay = p.keep - p.sinks - p.recent;            // of all candidates, this many stay
@@ -115,7 +114,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_rows_kernel(const __gri
       const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
       const uint32_t bits = digit == 2 ? 1023u : 2047u;
 #pragma unroll 4
-      for (int i = max(lo, 0) + tid; i < min(hi, mine); i += kSelThreads) {
+      for (int i = max(lo, 0) + tid; i < min(hi, mine); i += kThreads) {
         const uint32_t key = key_at(i);
         if ((key & known) == prefix) atomicAdd(&hist[0][(key >> shift) & bits], 1u);
       }
@@ -123,7 +122,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_rows_kernel(const __gri
       if (ctas > 1) {
         cluster.sync();
         const int slice = kSelBins / ctas;  // 2, 4 or 8 CTAs
-        for (int i = tid; i < slice; i += kSelThreads) {
+        for (int i = tid; i < slice; i += kThreads) {
           const int bin = rank_in * slice + i;
           uint32_t sum = 0;
           for (int r = 0; r < ctas; ++r) sum += cluster.map_shared_rank(hist[0], r)[bin];
@@ -134,9 +133,15 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_rows_kernel(const __gri
       } else {
         __syncthreads();
       }
-      // two bins a thread, from the highest down: their counts, then those above
-      const uint2 u = reinterpret_cast<const uint2 *>(total)[kSelBins / 2 - 1 - tid];
-      uint32_t inc = u.x + u.y;
+      // a few bins a thread, from the highest down: their counts, then those above
+      constexpr int kBins = kSelBins / kThreads;
+      uint32_t count[kBins], sum = 0;
+#pragma unroll
+      for (int j = 0; j < kBins; ++j) {
+        count[j] = total[kSelBins - 1 - kBins * tid - j];
+        sum += count[j];
+      }
+      uint32_t inc = sum;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
@@ -144,14 +149,19 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_rows_kernel(const __gri
       }
       if (lane == 31) warp_sum[warp] = inc;
       __syncthreads();
-      const uint32_t above = inc - (u.x + u.y) + __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0u);
-      if (above < rank && rank <= above + u.x + u.y) {
-        const bool second = rank > above + u.y;
-        pick_bin = kSelBins - 1 - 2 * tid - second;
-        pick_rank = rank - above - (second ? u.y : 0);
-        pick_count = second ? u.x : u.y;
+      uint32_t above = inc - sum + __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0u);
+      if (above < rank && rank <= above + sum) {
+#pragma unroll
+        for (int j = 0; j < kBins; ++j) {
+          if (above < rank && rank <= above + count[j]) {
+            pick_bin = kSelBins - 1 - kBins * tid - j;
+            pick_rank = rank - above;
+            pick_count = count[j];
+          }
+          above += count[j];
+        }
       }
-      for (int i = tid; i < kSelBins; i += kSelThreads) hist[0][i] = 0;
+      for (int i = tid; i < kSelBins; i += kThreads) hist[0][i] = 0;
       __syncthreads();
       prefix |= pick_bin << shift;
       known |= bits << shift;
@@ -222,7 +232,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_rows_kernel(const __gri
   int g0 = __reduce_add_sync(0xffffffffu, lane < warp ? n_gt[lane] : 0);
   int e0 = __reduce_add_sync(0xffffffffu, lane < warp ? n_eq[lane] : 0);
   if (ctas > 1) {
-    if (tid == kSelThreads - 1) {
+    if (tid == kThreads - 1) {
       cta_gt = g0 + gt;
       cta_eq = e0 + eq;
     }
@@ -256,7 +266,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_rows_kernel(const __gri
     }
   }
   if (ns)
-    for (int i = p.keep + rank_in * kSelThreads + tid; i < p.new_width; i += ctas * kSelThreads) ns[i] = 0.f;
+    for (int i = p.keep + rank_in * kThreads + tid; i < p.new_width; i += ctas * kThreads) ns[i] = 0.f;
   if (ctas > 1) cluster.sync();  // no CTA leaves while another may read its counts
 }
 

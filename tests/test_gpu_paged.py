@@ -486,9 +486,16 @@ def test_evict(rib, lib, dtype, D, nkv, page_rows, keep, sinks, recent):
                 sinks=sinks, recent=recent, extra=5)
 
 
-@pytest.mark.parametrize("n,keep", [(5000, 1234), (20001, 20000), (33000, 700)])
+@pytest.mark.parametrize("n,keep", [(1000, 300), (1900, 1899), (5000, 1234), (20001, 20000), (33000, 700), (280000, 1000)])
 def test_evict_long(rib, lib, n, keep):
     check_evict(rib, lib, [n, n // 3], nkv=2, D=64, page_rows=64, dtype=BF16, keep=keep, sinks=4, recent=keep // 8)
+
+
+def test_evict_many_heads(rib, lib):
+    """More (sequence, head) pairs than fit the GPU at once, of up to 1024 and up to 2048 rows."""
+    for high in (700, 1500):
+        check_evict(rib, lib, [high - 3 * b for b in range(100)], nkv=7, D=64, page_rows=64, dtype=BF16, keep=128, sinks=1,
+                    recent=16)
 
 
 def test_evict_ties_infinities_and_nan(rib, lib):
