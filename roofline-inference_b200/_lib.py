@@ -84,7 +84,8 @@ def _binding_command() -> list[str]:
     return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
             f"-I{sysconfig.get_paths()['include']}", f"-I{root / 'include'}",
             f"-I{root / 'include/torch/csrc/api/include'}", f"-I{Path(_nvcc()).resolve().parent.parent / 'include'}",
-            str(BINDING_SOURCE), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+            str(BINDING_SOURCE), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10",
+            "-lc10_cuda"]
 
 
 def binding_hash() -> str:
