@@ -57,10 +57,11 @@ int append_launch_lanes(rib::paged::AppendParams &p, cudaStream_t st) {
   if (!set_smem_once(append_kernel<T, LANES>, smem, g_append_smem_done[std::is_same<T, F16>::value][which]))
     return rib::host_fail(RIB_ECUDA, "cudaFuncSetAttribute(append smem)", smem);
   // As many lane groups to a token as one wave holds, a head each at most: few tokens spread over the
-  // GPU, many keep their cosines for all their heads.
+  // GPU, many keep their cosines for their heads.  Never fewer than two: the last, partly filled wave is
+  // half as long then (20000 tokens of 16 + 16 heads 70 us with one, 63 with two, 67 with four).
   constexpr int in_cta = kAppendThreads / LANES;
   const int items = p.nq + 2 * p.nkv, room = in_cta * kAppendCtas * sm_count();
-  p.groups = std::max(1, std::min(items, room / p.tokens));
+  p.groups = std::min(items, std::max(2, room / p.tokens));
   p.inv_dim = 1.0f / static_cast<float>(p.dim);
   const long long all = static_cast<long long>(p.tokens) * p.groups;
   return launch_pdl("append_kernel launch", append_kernel<T, LANES>, dim3(ceil_div(all, in_cta)), dim3(kAppendThreads),

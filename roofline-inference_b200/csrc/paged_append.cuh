@@ -14,10 +14,10 @@
 // sit in one lane and no lane exchanges dims with another (the norm's sum of squares is the only
 // shuffle).  A lane group keeps one token's cosines for all the heads it takes.  A row is short, so what
 // limits the kernel is how many are under way: each lane copies its next heads into a ring of its own
-// (cp.async), 4 ahead.  Measured on B200: 32768 tokens of 16 + 16 heads of 128 dims, normalised, in
-// 94-97 us (5.6 TB/s, 0.85 of the copy rate; loads into registers 119 us); 4093 tokens of 32 + 16 heads,
-// interleaved over 64 of 128 dims, 21 us (4.8 TB/s; with two chunks of neighbouring dims to a lane, half
-// a sector an access, 34 us); one token 2.9 us on the device.
+// (cp.async), 5 ahead.  Measured on B200: 32768 tokens of 16 + 16 heads of 128 dims, normalised, in
+// 91-93 us (5.8 TB/s, 0.89 of the copy rate; loads into registers 119 us); 4093 tokens of 32 + 16 heads,
+// interleaved over 64 of 128 dims, 20-21 us (4.9 TB/s; with two chunks of neighbouring dims to a lane,
+// half a sector an access, 34 us); one token 2.9 us on the device.
 #pragma once
 
 #include "paged_cache.cuh"
@@ -88,9 +88,9 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   return d;
 }
 
-constexpr int kAppendThreads = 128;
-constexpr int kAppendCtas = 4;    // resident per SM
-constexpr int kAppendStages = 5;  // heads of a lane that are under way
+constexpr int kAppendThreads = 64;  // small CTAs: a token ends without waiting for many others
+constexpr int kAppendCtas = 8;      // resident per SM
+constexpr int kAppendStages = 6;    // heads of a lane that are under way
 
 __device__ __forceinline__ void cp_async16(void *dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");

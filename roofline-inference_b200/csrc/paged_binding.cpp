@@ -373,10 +373,10 @@ PyObject *paged_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
                            step(scores, 0), step(scores, 1), keep, sinks, recent, rows.data_ptr<int32_t>(),
                            new_lens.data_ptr<int32_t>(), kept, kept_s[0], kept_s[1], kept_rows, stream_of(dev)),
             "paged_evict");
-    PyObject *pair = PyTuple_New(2);
-    if (!pair) return nullptr;
-    PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(rows));
-    PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(new_lens));
+    PyObject *first = THPVariable_Wrap(rows), *second = THPVariable_Wrap(new_lens);
+    PyObject *pair = first && second ? PyTuple_Pack(2, first, second) : nullptr;
+    Py_XDECREF(first);
+    Py_XDECREF(second);
     return pair;
   });
 }
