@@ -88,7 +88,9 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   return d;
 }
 
-constexpr int kAppendThreads = 64;  // small CTAs: a token ends without waiting for many others
+// 32768 tokens: 92.0 us with 5 stages, 91.2 with 6, 90.6 with 9 (which costs short calls); 94.1 with CTAs
+// of 128 threads.
+constexpr int kAppendThreads = 64;
 constexpr int kAppendCtas = 8;      // resident per SM
 constexpr int kAppendStages = 6;    // heads of a lane that are under way
 

@@ -41,7 +41,9 @@ constexpr int TK = 16;        // rows of a tile: one TMA box, one page at most
 constexpr int NW = 4;         // warps of a CTA
 constexpr int NT = NW * 32;
 constexpr int HU = 8;         // query heads of a unit
-constexpr int kMinTiles = 8;  // tiles of a piece where CTAs idle: two for each warp
+// Tiles of a piece where CTAs idle: two for each warp (8 x 512 rows 9.2 us, with 4 tiles 9.9; 1 x 513 rows
+// 7.3, with 4 tiles 7.0, with 16 10.1).
+constexpr int kMinTiles = 8;
 // Where no sequence can have more rows than this, units stay whole and nothing is launched to join them
 // (8 x 256 rows: 7.3 us, split and joined 8.4; 64 x 100-200 rows: 13.9, 17.4.  With 512 rows it depends
 // on the batch: 64 sequences 25.4 whole, 28.6 split, 8 sequences 11.0 and 9.2).

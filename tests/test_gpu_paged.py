@@ -588,6 +588,57 @@ def test_outputs_that_overlap_are_refused(rib, lib):
     assert lib.take_device_status() == 0
 
 
+@pytest.mark.parametrize("n,keep", [(900, 300), (5000, 700), (70000, 5000)])
+def test_evict_captured_and_on_two_streams(rib, lib, n, keep):
+    """A captured eviction replays with what its buffers hold, while another runs on its own stream."""
+    g = gen(21)
+    nkv, D, P = 2, 64, 64
+
+    def state(seed):
+        s = gen(seed)
+        pages, table = make_cache([n], nkv, D, P, BF16, s, spare=-(-keep // P), fill=0.25)
+        free = sorted(set(range(pages.shape[0])) - set(table.flatten().tolist()))
+        return dict(pages=pages, table=table, lens=i32([n]), new=i32([free]), kept=torch.zeros((1, nkv, keep), device="cuda"),
+                    scores=torch.zeros((1, nkv, table.shape[1] * P), device="cuda"))
+
+    def call(st):
+        return rib.paged_evict(st["pages"], st["table"], st["lens"], st["scores"], keep, st["new"], sinks=2, recent=9,
+                               new_scores=st["kept"])
+    states, graphs, outs = [state(1), state(2)], [], []
+    for st in states:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call(st)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(call(st))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for step in range(3):
+        lens = [n - 7 * step, keep + step]
+        inputs = [torch.randn((1, nkv, states[0]["scores"].shape[2]), generator=g).cuda() for _ in states]
+        torch.cuda.synchronize()
+        for st, graph, stream, x, m in zip(states, graphs, streams, inputs, lens):
+            with torch.cuda.stream(stream):
+                st["scores"].copy_(x)
+                st["lens"].fill_(m)
+                graph.replay()
+        torch.cuda.synchronize()
+        for st, (rows, new_lens), x, m in zip(states, outs, inputs, lens):
+            assert new_lens.tolist() == [min(m, keep)]
+            for h in range(nkv):
+                at = kept_rows(x[0, h].cpu(), m, keep, 2, 9)
+                assert rows[0, h].tolist() == at
+                at = torch.tensor(at, device="cuda")
+                to = torch.arange(keep, device="cuda")
+                assert torch.equal(st["pages"][st["new"][0, to // P].long(), :, h, to % P],
+                                   st["pages"][st["table"][0, at // P].long(), :, h, at % P])
+                assert torch.equal(st["kept"][0, h], x[0, h, at])
+    assert lib.take_device_status() == 0
+
+
 def test_evict_reports_missing_pages(rib, lib):
     g = gen(2)
     pages, table = make_cache([64], 1, 64, 16, BF16, g, spare=2, fill=0.0)
