@@ -4,6 +4,10 @@
 // every dimension but the last; `table` [seqs][width] names the pages of each sequence in order, so
 // row r of sequence s lies in page table[s][r / page_rows] at r % page_rows.  A table entry outside
 // [0, num_pages) names no page: no kernel reads or writes through it.
+//
+// Every kernel here waits for the one before it (pdl_wait) before it touches memory, and reads what that
+// one may have written with ordinary loads: it may be running while the other still writes, so nothing
+// is read-only for its whole life, as the non-coherent path asks.
 #pragma once
 
 #include "common.cuh"
@@ -39,7 +43,7 @@ struct F16 {
 __device__ __forceinline__ int page_of(const View &v, int s, int r) {
   const int i = r / v.page_rows;
   if (s < 0 || s >= v.seqs || r < 0 || i >= v.width) return -1;
-  const int page = __ldg(v.table + s * v.table_stride + i);
+  const int page = v.table[s * v.table_stride + i];
   return page >= 0 && page < v.num_pages ? page : -1;
 }
 

@@ -146,7 +146,7 @@ __device__ __forceinline__ void mma16816<F16>(float (&c)[4], uint32_t a0, uint32
 
 // Rows of sequence b that are attended: lens[b] within what the table and the caller's bound hold.
 __device__ __forceinline__ int seq_rows(const DecodeParams &p, int b) {
-  const int n = __ldg(p.lens + b);
+  const int n = p.lens[b];
   return n < 0 ? 0 : n < p.max_len ? n : p.max_len;
 }
 __device__ __forceinline__ int seq_tiles(const DecodeParams &p, int b) { return (seq_rows(p, b) + TK - 1) / TK; }
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(NT, DecodeCfg<D>::CTAS) paged_decode_kernel(co
     }
   };
   auto page_at = [&](const Place &pl) {
-    return __ldg(p.cache.table + pl.b * p.cache.table_stride + pl.tile * TK / p.cache.page_rows);
+    return p.cache.table[pl.b * p.cache.table_stride + pl.tile * TK / p.cache.page_rows];
   };
   auto copy = [&](const Place &pl, int page, int slot) {
     if (page < 0 || page >= p.cache.num_pages) {
@@ -361,8 +361,8 @@ __global__ void __launch_bounds__(NT, DecodeCfg<D>::CTAS) paged_decode_kernel(co
       const uint16_t *qr = p.q + c.b * p.q_seq + (h0 + g) * p.q_head + 2 * t4;
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) {
-        qa[s][0] = g < heads ? __ldg(reinterpret_cast<const uint32_t *>(qr + 16 * s)) : 0u;
-        qa[s][1] = g < heads ? __ldg(reinterpret_cast<const uint32_t *>(qr + 16 * s + 8)) : 0u;
+        qa[s][0] = g < heads ? *reinterpret_cast<const uint32_t *>(qr + 16 * s) : 0u;
+        qa[s][1] = g < heads ? *reinterpret_cast<const uint32_t *>(qr + 16 * s + 8) : 0u;
       }
     }
     float m = -INFINITY, l = 0.f;
