@@ -192,13 +192,15 @@ int select_launch(const rib::paged::SelectParams &s, long long units, int batch,
   while (ctas < 8 && 2 * ctas * units <= sm_count() && s.max_len >= 8192 * ctas) ctas *= 2;
   const int part = ceil_div(s.max_len, ctas * kThreads) * kThreads;
   constexpr int most = kSelStepRows * kThreads;
-  const bool fits = part <= most;
+  const bool fits = part <= most;  // always with 512 threads
   if (!set_smem_once(select_rows_kernel<kThreads, true>, most * static_cast<int>(sizeof(float)),
                      g_select_smem_done[kThreads == 1024]))
     return rib::host_fail(RIB_ECUDA, "cudaFuncSetAttribute(select smem)", most);
-  return launch_cluster("select_rows_kernel launch",
-                        fits ? select_rows_kernel<kThreads, true> : select_rows_kernel<kThreads, false>,
-                        dim3(s.nkv * ctas, batch), dim3(kThreads), fits ? part * sizeof(float) : 0, ctas, st, s);
+  auto kernel = select_rows_kernel<kThreads, true>;
+  if constexpr (kThreads == 1024)
+    if (!fits) kernel = select_rows_kernel<kThreads, false>;
+  return launch_cluster("select_rows_kernel launch", kernel, dim3(s.nkv * ctas, batch), dim3(kThreads),
+                        fits ? part * sizeof(float) : 0, ctas, st, s);
 }
 
 }  // namespace

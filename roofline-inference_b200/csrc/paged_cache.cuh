@@ -27,16 +27,14 @@ struct View {
 struct BF16 {
   static __device__ __forceinline__ float2 unpack(uint32_t w) { return make_float2(bf16lo(w), bf16hi(w)); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
-  static __device__ __forceinline__ float one(uint16_t v) { return bf16lo(v); }
-  static constexpr int kLift = 0;   // a weight in (0, 1] keeps its precision down to 2^-126
+  static constexpr int kLift = 0;   // a weight in (0, 1] keeps its relative precision down to 2^-126
 };
 struct F16 {
   static __device__ __forceinline__ float2 unpack(uint32_t w) {
     return __half22float2(*reinterpret_cast<const __half2 *>(&w));
   }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_f16x2(lo, hi); }
-  static __device__ __forceinline__ float one(uint16_t v) { return __half2float(__ushort_as_half(v)); }
-  static constexpr int kLift = 14;  // times 2^14, a weight in (0, 1] does down to 2^-28, and is exact to 2^-38
+  static constexpr int kLift = 14;  // times 2^14, it does down to 2^-28, and below that is off by 2^-39 at most
 };
 
 // Page of row `r` of sequence `s`, or -1 where the table names none.
