@@ -108,9 +108,9 @@ PagedDecodeLayout paged_decode_layout(int batch, int max_len, int nq, int dim, b
   using namespace rib::paged;
   PagedDecodeLayout l;
   l.grid = (dim == 128 ? DecodeCfg<128>::CTAS : DecodeCfg<64>::CTAS) * sm_count();
-  size_t off = round256(static_cast<size_t>(l.grid) * 2 * HU * dim * sizeof(float));
+  size_t off = round256(static_cast<size_t>(l.grid) * 2 * kMaxUnitHeads * dim * sizeof(float));
   l.ml_off = off;
-  off += round256(static_cast<size_t>(l.grid) * 2 * HU * 2 * sizeof(float));
+  off += round256(static_cast<size_t>(l.grid) * 2 * kMaxUnitHeads * 2 * sizeof(float));
   l.rec_off = off;
   off += round256(static_cast<size_t>(l.grid) * sizeof(JoinRecord));
   l.logit_row = (static_cast<long long>(max_len) + TK - 1) / TK * TK;
@@ -148,15 +148,15 @@ bool paged_map(CUtensorMap *m, const rib_paged_cache *c) {
   return r == CUDA_SUCCESS;
 }
 
-bool g_paged_smem_done[2][2][2][kMaxDevices];
+bool g_paged_smem_done[2][2][2][2][kMaxDevices];
 bool g_select_smem_done[2][kMaxDevices];
 
-template <class T, int D, bool kLogits>
+template <class T, int D, int HU, bool kLogits>
 int paged_decode_launch(const rib::paged::DecodeParams &p, int grid, cudaStream_t st) {
   using namespace rib::paged;
-  auto kernel = paged_decode_kernel<T, D, kLogits>;
-  const int smem = static_cast<int>(sizeof(DecodeSmem<D>)) + 1024;
-  if (!set_smem_once(kernel, smem, g_paged_smem_done[std::is_same<T, F16>::value][D == 128][kLogits]))
+  auto kernel = paged_decode_kernel<T, D, HU, kLogits>;
+  const int smem = static_cast<int>(sizeof(DecodeSmem<D, HU>)) + 1024;
+  if (!set_smem_once(kernel, smem, g_paged_smem_done[std::is_same<T, F16>::value][D == 128][HU == 16][kLogits]))
     return rib::host_fail(RIB_ECUDA, "cudaFuncSetAttribute(paged decode smem)", smem);
   const int s = launch_pdl("paged_decode_kernel launch", kernel, dim3(grid), dim3(NT), smem, st, p);
   if (s != RIB_OK || (p.whole && !kLogits)) return s;
@@ -171,15 +171,27 @@ int paged_decode_launch(const rib::paged::DecodeParams &p, int grid, cudaStream_
   }
   const long long blocks = grid + row_blocks * heads;
   if (blocks > 0x7fffffffLL) return RIB_EINVAL;
-  return launch_pdl("join_kernel launch", join_kernel<T, D>, dim3(static_cast<unsigned>(blocks)), dim3(kJoinThreads), 0,
+  return launch_pdl("join_kernel launch", join_kernel<T, D, HU>, dim3(static_cast<unsigned>(blocks)), dim3(kJoinThreads), 0,
                     st, p, grid, row_blocks, rows);
 }
 
-template <class T>
+template <class T, int HU>
 int paged_decode_launch(const rib::paged::DecodeParams &p, int dim, int grid, cudaStream_t st) {
   if (dim == 128)
-    return p.logits ? paged_decode_launch<T, 128, true>(p, grid, st) : paged_decode_launch<T, 128, false>(p, grid, st);
-  return p.logits ? paged_decode_launch<T, 64, true>(p, grid, st) : paged_decode_launch<T, 64, false>(p, grid, st);
+    return p.logits ? paged_decode_launch<T, 128, HU, true>(p, grid, st)
+                    : paged_decode_launch<T, 128, HU, false>(p, grid, st);
+  return p.logits ? paged_decode_launch<T, 64, HU, true>(p, grid, st) : paged_decode_launch<T, 64, HU, false>(p, grid, st);
+}
+
+// Units of 8 query heads, or of 16 where a KV head has more than 8: its rows are read once per unit (64 x
+// 8-9k rows, 16 heads over one of 128 dims: 52 us, as two units of 8 88; with 8 heads, 16 would do twice
+// the P.V products for nothing).
+inline int unit_heads(int group) { return group <= 8 ? 8 : 16; }
+
+template <class T>
+int paged_decode_launch(const rib::paged::DecodeParams &p, int dim, int grid, cudaStream_t st) {
+  return unit_heads(p.group) == 8 ? paged_decode_launch<T, 8>(p, dim, grid, st)
+                                  : paged_decode_launch<T, 16>(p, dim, grid, st);
 }
 
 template <int kThreads>
@@ -321,7 +333,7 @@ int rib_paged_decode_attention(const rib_paged_cache *cache, const void *q, long
   p.batch = batch;
   p.nq = nq;
   p.group = nq / cache->nkv;
-  p.units_per_kv = ceil_div(p.group, HU);
+  p.units_per_kv = ceil_div(p.group, unit_heads(p.group));
   p.max_len = max_len;
   p.scale2 = static_cast<float>(scale * 1.4426950408889634);
   p.whole = max_len <= kWholeRows;

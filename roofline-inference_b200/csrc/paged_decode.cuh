@@ -5,7 +5,7 @@
 // weight that each row of each KV head received, w[b][kvh][n] = sum over the head's query heads of
 // p_hn, is added to a score per row (what an eviction goes by).
 //
-// Work split: the unit is (sequence, KV head, 8 query heads).  The tiles of TK rows of all units lie
+// Work split: the unit is (sequence, KV head, HU = 8 or 16 query heads).  The tiles of TK rows of all units lie
 // on one line, unit after unit, and every CTA of one wave takes an equal run of them, found from the
 // lengths on the device: ragged batches and single long sequences fill the GPU alike, and the host
 // never needs the lengths.  A CTA writes the units that lie wholly in its run, and one partial
@@ -19,10 +19,11 @@
 // the heads as the 16 rows.  A decode step reads 4 D bytes per row for 4 D flops per query head, so
 // memory bounds it at any group size here (8 heads per KV head: 52 TFLOP/s at the full memory rate), and
 // a tcgen05 tile (128 rows at least, accumulators in TMEM) would add a round trip through TMEM for rows
-// that stay empty.  The upper 8 rows of the A operand are free with 8 heads: in P.V they carry
+// that stay empty.  With 8 heads the upper 8 rows of the A operand are free: in P.V they carry
 // p - round(p), so P enters with 16 (BF16) or 22 (FP16) bits and its rounding adds nothing to the
 // output's.  FP16 weights are lifted by 2^14 (as is their sum), out of the type's subnormal range: many
-// small weights behind one large one add up.
+// small weights behind one large one add up.  With more than 8 heads per KV head all 16 rows are heads, so
+// the rows are still read once, and the rounding's part is a second mma.
 //
 // Measured on B200 (one launch pair, state larger than L2): 64 sequences of 30-33k rows, 8 KV heads of
 // 64 dims, 605-633 us (6.5-6.8 TB/s); 32 x 8191 rows, 64 heads over 8, FP16, 165-169 us (6.4-6.5 TB/s,
@@ -40,7 +41,7 @@ namespace paged {
 constexpr int TK = 16;        // rows of a tile: one TMA box, one page at most
 constexpr int NW = 4;         // warps of a CTA
 constexpr int NT = NW * 32;
-constexpr int HU = 8;         // query heads of a unit
+constexpr int kMaxUnitHeads = 16;  // query heads of a unit at most
 // Tiles of a piece where CTAs idle: two for each warp (8 x 512 rows 9.2 us, with 4 tiles 9.9; 1 x 513 rows
 // 7.3, with 4 tiles 7.0, with 16 10.1).
 constexpr int kMinTiles = 8;
@@ -59,7 +60,7 @@ struct DecodeCfg {
   static constexpr int STAGE = HALF * (D / 64);
 };
 
-template <int D>
+template <int D, int HU>
 struct DecodeSmem {
   alignas(1024) uint8_t ring[NW][DecodeCfg<D>::ST][DecodeCfg<D>::STAGE];
   // [warp that sums][the others][head][its share of the dims], rows padded against bank conflicts
@@ -86,7 +87,7 @@ struct DecodeParams {
   int batch, nq, group, units_per_kv;
   int max_len;                  // rows a sequence may have (host bound)
   float scale2;                 // scale * log2 e
-  float *part_o;                // [grid][2][HU][D]
+  float *part_o;                // [grid][2][HU][D], HU the query heads of a unit (8 or 16)
   float *part_ml;               // [grid][2][HU][2]
   JoinRecord *rec;              // [grid]
   float *logits;                // [B][nq][logit_row] scores in log2 units, or null
@@ -176,12 +177,13 @@ __device__ __forceinline__ float2 weight_norm(float M, float L) {
   return make_float2(M, static_cast<float>(1 << T::kLift) / L);
 }
 
-template <class T, int D, bool kLogits>
+template <class T, int D, int HU, bool kLogits>
 __global__ void __launch_bounds__(NT, DecodeCfg<D>::CTAS) paged_decode_kernel(const __grid_constant__ DecodeParams p) {
   using Cfg = DecodeCfg<D>;
+  constexpr int R = HU / 8;  // heads of a lane: rows g and, with 16 heads, g + 8 of the mma tiles
   constexpr int ST = Cfg::ST;
   extern __shared__ uint8_t smem_raw[];
-  DecodeSmem<D> &sm = *reinterpret_cast<DecodeSmem<D> *>(
+  DecodeSmem<D, HU> &sm = *reinterpret_cast<DecodeSmem<D, HU> *>(
       smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int units = p.cache.nkv * p.units_per_kv;
@@ -355,17 +357,23 @@ __global__ void __launch_bounds__(NT, DecodeCfg<D>::CTAS) paged_decode_kernel(co
     const int seg = min(c.tiles - c.tile, run - f);
     const int kvh = c.hu / p.units_per_kv, g0 = (c.hu % p.units_per_kv) * HU;
     const int heads = min(HU, p.group - g0), h0 = kvh * p.group + g0;
-    // A fragments of q: lane row g is head h0 + g, rows 8-15 are zero
-    uint32_t qa[D / 16][2];
-    {
-      const uint16_t *qr = p.q + c.b * p.q_seq + (h0 + g) * p.q_head + 2 * t4;
+    // A fragments of q: rows g (and g + 8) are heads h0 + g (and h0 + g + 8), the others zero
+    uint32_t qa[R][D / 16][2];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const uint16_t *qr = p.q + c.b * p.q_seq + (h0 + g + 8 * r) * p.q_head + 2 * t4;
 #pragma unroll
       for (int s = 0; s < D / 16; ++s) {
-        qa[s][0] = g < heads ? *reinterpret_cast<const uint32_t *>(qr + 16 * s) : 0u;
-        qa[s][1] = g < heads ? *reinterpret_cast<const uint32_t *>(qr + 16 * s + 8) : 0u;
+        qa[r][s][0] = g + 8 * r < heads ? *reinterpret_cast<const uint32_t *>(qr + 16 * s) : 0u;
+        qa[r][s][1] = g + 8 * r < heads ? *reinterpret_cast<const uint32_t *>(qr + 16 * s + 8) : 0u;
       }
     }
-    float m = -INFINITY, l = 0.f;
+    float m[R], l[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      m[r] = -INFINITY;
+      l[r] = 0.f;
+    }
     float o[D / 8][4];
 #pragma unroll
     for (int i = 0; i < D / 8; ++i)
@@ -401,112 +409,144 @@ __global__ void __launch_bounds__(NT, DecodeCfg<D>::CTAS) paged_decode_kernel(co
           const int cc = ch + (lane >> 3);
           uint32_t kb[4];
           ldsm4(base + (cc >> 3) * Cfg::HALF + r * 128 + (((cc & 7) ^ (r & 7)) << 4), kb);
-          mma16816<T>(s[nt], qa[ch / 2][0], 0u, qa[ch / 2][1], 0u, kb[0], kb[1]);
-          mma16816<T>(s_odd, qa[ch / 2 + 1][0], 0u, qa[ch / 2 + 1][1], 0u, kb[2], kb[3]);
+          const int e = ch / 2;
+          mma16816<T>(s[nt], qa[0][e][0], R > 1 ? qa[R - 1][e][0] : 0u, qa[0][e][1], R > 1 ? qa[R - 1][e][1] : 0u, kb[0],
+                      kb[1]);
+          mma16816<T>(s_odd, qa[0][e + 1][0], R > 1 ? qa[R - 1][e + 1][0] : 0u, qa[0][e + 1][1],
+                      R > 1 ? qa[R - 1][e + 1][1] : 0u, kb[2], kb[3]);
         }
-        s[nt][0] += s_odd[0];
-        s[nt][1] += s_odd[1];
-      }
-      // ---- softmax in log2 units; lane holds rows 2 t4, 2 t4 + 1 of both n-tiles for head g
-      float sc[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = (e >> 1) * 8 + 2 * t4 + (e & 1);
-        sc[e] = r < rows ? s[e >> 1][e & 1] * p.scale2 : -INFINITY;
+        for (int e = 0; e < 2 * R; ++e) s[nt][e] += s_odd[e];
       }
-      if (kLogits && g < heads) {
-        float *lg = p.logits + (static_cast<size_t>(c.b) * p.nq + h0 + g) * p.logit_row + k0 + 2 * t4;
-        *reinterpret_cast<float2 *>(lg) = make_float2(sc[0], sc[1]);
-        *reinterpret_cast<float2 *>(lg + 8) = make_float2(sc[2], sc[3]);
+      // ---- softmax in log2 units; lane holds rows 2 t4, 2 t4 + 1 of both n-tiles for each of its heads
+      float pr[R][4];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float sc[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = (e >> 1) * 8 + 2 * t4 + (e & 1);
+          sc[e] = row < rows ? s[e >> 1][2 * r + (e & 1)] * p.scale2 : -INFINITY;
+        }
+        if (kLogits && g + 8 * r < heads) {
+          float *lg = p.logits + (static_cast<size_t>(c.b) * p.nq + h0 + g + 8 * r) * p.logit_row + k0 + 2 * t4;
+          *reinterpret_cast<float2 *>(lg) = make_float2(sc[0], sc[1]);
+          *reinterpret_cast<float2 *>(lg + 8) = make_float2(sc[2], sc[3]);
+        }
+        float mt = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+        mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+        mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
+        const float mn = fmaxf(m[r], mt);
+        const float mz = mn == -INFINITY ? 0.f : mn;  // every score -inf so far: weights 0, not exp(inf - inf)
+        if (__any_sync(0xffffffffu, mn != m[r])) {
+          const float al = fast_exp2(m[r] - mz);
+          l[r] *= al;
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+            for (int e = 2 * r; e < (R > 1 ? 2 * r + 2 : 4); ++e) o[i][e] *= al;
+          m[r] = mn;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pr[r][e] = fast_exp2(T::kLift ? sc[e] - mz + T::kLift : sc[e] - mz);
+        l[r] += (pr[r][0] + pr[r][1]) + (pr[r][2] + pr[r][3]);
       }
-      float mt = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
-      mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
-      mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
-      const float mn = fmaxf(m, mt);
-      const float mz = mn == -INFINITY ? 0.f : mn;  // every score -inf so far: weights 0, not exp(inf - inf)
-      if (__any_sync(0xffffffffu, mn != m)) {
-        const float al = fast_exp2(m - mz);
-        l *= al;
+      // A fragments of P: the rounded weights, and what the rounding left (with 8 heads in rows 8-15)
+      uint32_t hi[R][2], lo[R][2];
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i)
+      for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[i][e] *= al;
-        m = mn;
-      }
-      float pr[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) pr[e] = fast_exp2(T::kLift ? sc[e] - mz + T::kLift : sc[e] - mz);
-      l += (pr[0] + pr[1]) + (pr[2] + pr[3]);
-      // A fragments of P: rows 0-7 the rounded weights, rows 8-15 what the rounding left
-      const uint32_t a0 = T::pack(pr[0], pr[1]), a2 = T::pack(pr[2], pr[3]);
-      const float2 f0 = T::unpack(a0), f2 = T::unpack(a2);
-      const uint32_t a1 = T::pack(pr[0] - f0.x, pr[1] - f0.y), a3 = T::pack(pr[2] - f2.x, pr[3] - f2.y);
+        for (int e = 0; e < 2; ++e) {
+          hi[r][e] = T::pack(pr[r][2 * e], pr[r][2 * e + 1]);
+          const float2 f = T::unpack(hi[r][e]);
+          lo[r][e] = T::pack(pr[r][2 * e] - f.x, pr[r][2 * e + 1] - f.y);
+        }
 #pragma unroll
       for (int ch = 0; ch < D / 8; ch += 2) {
         const int r = lane & 15, cc = ch + (lane >> 4);
         uint32_t vb[4];
         ldsm4_t(base + (cc >> 3) * Cfg::HALF + (TK + r) * 128 + (((cc & 7) ^ (r & 7)) << 4), vb);
-        mma16816<T>(o[ch], a0, a1, a2, a3, vb[0], vb[1]);
-        mma16816<T>(o[ch + 1], a0, a1, a2, a3, vb[2], vb[3]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (R > 1) {
+            mma16816<T>(o[ch + e], hi[0][0], hi[R - 1][0], hi[0][1], hi[R - 1][1], vb[2 * e], vb[2 * e + 1]);
+            mma16816<T>(o[ch + e], lo[0][0], lo[R - 1][0], lo[0][1], lo[R - 1][1], vb[2 * e], vb[2 * e + 1]);
+          } else {
+            mma16816<T>(o[ch + e], hi[0][0], lo[0][0], hi[0][1], lo[0][1], vb[2 * e], vb[2 * e + 1]);
+          }
+        }
       }
       __syncwarp();  // every lane has read the slot
       if (lane == 0 && issued < count) issue();
     }
 
     // ---- the warps' results of this unit: scaled to a common maximum, summed in warp order
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if (t4 == 0) sm.m[warp][g] = m;
-    __syncthreads();
-    float M = sm.m[0][g];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) M = fmaxf(M, sm.m[w][g]);
-    const float al = M == -INFINITY ? 0.f : fast_exp2(m - M);
-    if (t4 == 0) sm.l[warp][g] = l * al;
+    for (int r = 0; r < R; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      if (t4 == 0) sm.m[warp][g + 8 * r] = m[r];
+    }
+    __syncthreads();
     // every warp sums a share of the dims: it keeps its own part of those and hands out the rest
     constexpr int S = D / 8 / NW;  // n-tiles of a share
-    float2 own[S];
+    float2 own[R][S];
+    float M[R];
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-      const float2 v = make_float2((o[i][0] + o[i][2]) * al, (o[i][1] + o[i][3]) * al);
-      if (i / S == warp)
-        own[i % S] = v;
-      else
-        *reinterpret_cast<float2 *>(&sm.o[i / S][warp - (warp > i / S)][g][i % S * 8 + 2 * t4]) = v;
+    for (int r = 0; r < R; ++r) {
+      M[r] = sm.m[0][g + 8 * r];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) M[r] = fmaxf(M[r], sm.m[w][g + 8 * r]);
+      const float al = M[r] == -INFINITY ? 0.f : fast_exp2(m[r] - M[r]);
+      if (t4 == 0) sm.l[warp][g + 8 * r] = l[r] * al;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        const float2 v = R > 1 ? make_float2(o[i][2 * r] * al, o[i][2 * r + 1] * al)
+                               : make_float2((o[i][0] + o[i][2]) * al, (o[i][1] + o[i][3]) * al);
+        if (i / S == warp)
+          own[r][i % S] = v;
+        else
+          *reinterpret_cast<float2 *>(&sm.o[i / S][warp - (warp > i / S)][g + 8 * r][i % S * 8 + 2 * t4]) = v;
+      }
     }
     __syncthreads();
     {
-      float L = sm.l[0][g];
-#pragma unroll
-      for (int w = 1; w < NW; ++w) L += sm.l[w][g];
       const bool whole = c.tile == 0 && seg == c.tiles;
       const int part = c.tile > 0 ? 0 : 1;
-      const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);  // a NaN sum stays NaN
       const int d0 = warp * (D / NW) + 2 * t4;
-      uint16_t *out = p.out + (static_cast<size_t>(c.b) * p.nq + h0 + g) * D + d0;
-      float *po = p.part_o + ((static_cast<size_t>(cta) * 2 + part) * HU + g) * D + d0;
 #pragma unroll
-      for (int i = 0; i < S; ++i) {
-        float2 v = make_float2(0.f, 0.f);  // in warp order
+      for (int r = 0; r < R; ++r) {
+        const int hd = g + 8 * r;
+        float L = sm.l[0][hd];
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-          const float2 u = w == warp ? own[i]
-                                     : *reinterpret_cast<const float2 *>(&sm.o[warp][w - (w > warp)][g][i * 8 + 2 * t4]);
-          v.x += u.x;
-          v.y += u.y;
+        for (int w = 1; w < NW; ++w) L += sm.l[w][hd];
+        const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);  // a NaN sum stays NaN
+        uint16_t *out = p.out + (static_cast<size_t>(c.b) * p.nq + h0 + hd) * D + d0;
+        float *po = p.part_o + ((static_cast<size_t>(cta) * 2 + part) * HU + hd) * D + d0;
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+          float2 v = make_float2(0.f, 0.f);  // in warp order
+#pragma unroll
+          for (int w = 0; w < NW; ++w) {
+            const float2 u = w == warp ? own[r][i]
+                                       : *reinterpret_cast<const float2 *>(&sm.o[warp][w - (w > warp)][hd][i * 8 + 2 * t4]);
+            v.x += u.x;
+            v.y += u.y;
+          }
+          if (hd < heads) {
+            if (whole)
+              *reinterpret_cast<uint32_t *>(out + 8 * i) = T::pack(v.x * inv, v.y * inv);
+            else
+              *reinterpret_cast<float2 *>(po + 8 * i) = v;
+          }
         }
-        if (g < heads) {
-          if (whole)
-            *reinterpret_cast<uint32_t *>(out + 8 * i) = T::pack(v.x * inv, v.y * inv);
-          else
-            *reinterpret_cast<float2 *>(po + 8 * i) = v;
+        if (warp == 0 && t4 == 0 && hd < heads) {
+          if (!whole)
+            *reinterpret_cast<float2 *>(p.part_ml + ((static_cast<size_t>(cta) * 2 + part) * HU + hd) * 2) =
+                make_float2(M[r], L);
+          else if (kLogits)
+            p.norm[static_cast<size_t>(c.b) * p.nq + h0 + hd] = weight_norm<T>(M[r], L);
         }
-      }
-      if (warp == 0 && t4 == 0 && g < heads) {
-        if (!whole)
-          *reinterpret_cast<float2 *>(p.part_ml + ((static_cast<size_t>(cta) * 2 + part) * HU + g) * 2) = make_float2(M, L);
-        else if (kLogits)
-          p.norm[static_cast<size_t>(c.b) * p.nq + h0 + g] = weight_norm<T>(M, L);
       }
       if (tid == 0) {
         int last = -1;  // the CTA in which a unit that begins here and does not end here ends
@@ -528,12 +568,14 @@ __global__ void __launch_bounds__(NT, DecodeCfg<D>::CTAS) paged_decode_kernel(co
 }
 
 constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * 32;
+constexpr int kNormHeads = 128;  // heads whose row weights are summed at once
 
 // Place of CTA c's partial of a unit that begins in CTA `first`: that one's second, the others' first.
 __device__ __forceinline__ size_t part_slot(int c, int first) { return static_cast<size_t>(c) * 2 + (c == first); }
 
 // Maximum and sum of head g of a unit over its partials, by a whole warp (in every lane, in CTA order
 // within a lane and by a fixed tree over the lanes).
+template <int HU>
 __device__ __forceinline__ float2 joined_ml(const DecodeParams &p, int first, int last, int g, int lane) {
   float M = -INFINITY, L = 0.f;
   for (int c = first + lane; c <= last; c += 32) {
@@ -555,12 +597,13 @@ __device__ __forceinline__ float2 joined_ml(const DecodeParams &p, int first, in
 // Blocks below `grid`: join the unit that begins in that CTA's run and ends in another's.  The warps
 // take (head, slice of the partials), so all partials are under way at once; the slices are summed in
 // order.  With scores, the blocks behind add the row weights, `rows` rows of one KV head each.
-template <class T, int D>
+template <class T, int D, int HU>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ DecodeParams p, int grid,
                                                             int row_blocks, int rows) {
-  __shared__ float4 acc[kJoinWarps][D / 4];
-  __shared__ float head_sum[kJoinWarps];
-  __shared__ float2 head_norm[kJoinWarps];
+  constexpr int kSums = HU > kJoinWarps ? HU : kJoinWarps;
+  __shared__ float4 acc[kSums][D / 4];  // [head][slice]
+  __shared__ float head_sum[HU];
+  __shared__ float2 head_norm[kNormHeads];
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -569,11 +612,11 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     if (r.last < 0) return;
     const int first = blockIdx.x, kvh = r.hu / p.units_per_kv, g0 = (r.hu % p.units_per_kv) * HU;
     const int heads = min(HU, p.group - g0), h0 = kvh * p.group + g0;
-    const int slices = kJoinWarps / heads, g = warp / slices, slice = warp % slices;
+    const int slices = heads < kJoinWarps ? kJoinWarps / heads : 1, slice = warp % slices;
     constexpr int V = D / 4, R = 32 / V;  // lanes of a row, rows of a load
     constexpr int N = D == 128 ? 6 : 4;   // loads under way at once
     const int v = lane % V, step = slices * R;
-    if (g < heads) {
+    for (int g = warp / slices; g < heads; g += kJoinWarps / slices) {
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
       float2 all = make_float2(0.f, 0.f);
       for (int c0 = first + slice * R + lane / V; c0 - lane / V <= r.last; c0 += N * step) {
@@ -587,7 +630,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
           u[i] = *reinterpret_cast<const float4 *>(p.part_o + s * D + 4 * v);
           m[i] = p.part_ml[2 * s];
         }
-        if (c0 - lane / V == first + slice * R) all = joined_ml(p, first, r.last, g, lane);
+        if (c0 - lane / V == first + slice * R) all = joined_ml<HU>(p, first, r.last, g, lane);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           if (c0 + i * step > r.last) continue;
@@ -604,7 +647,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
         o.z += __shfl_xor_sync(0xffffffffu, o.z, 16);
         o.w += __shfl_xor_sync(0xffffffffu, o.w, 16);
       }
-      if (lane < V) acc[warp][v] = o;
+      if (lane < V) acc[g * slices + slice][v] = o;
       if (lane == 0 && slice == 0) head_sum[g] = all.y;
     }
     __syncthreads();
@@ -628,45 +671,53 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   const int n = min(rows, seq_rows(p, b) - k0);
   if (n <= 0) return;
   float *out = p.scores_out + b * p.out_seq + h * p.out_head + k0;
-  for (int u = 0; u < p.units_per_kv; ++u) {
-    const int hu = h * p.units_per_kv + u, heads = min(HU, p.group - u * HU);
-    const size_t head0 = static_cast<size_t>(b) * p.nq + h * p.group + u * HU;
-    if (warp < heads) {
-      const int2 span = p.span[static_cast<size_t>(b) * p.cache.nkv * p.units_per_kv + hu];
+  const size_t first_head = static_cast<size_t>(b) * p.nq + h * p.group;
+  // all heads' weights of a row are summed before the score is touched (beyond kNormHeads heads, in parts)
+  for (int part = 0; part < p.group; part += kNormHeads) {
+    const int heads = min(kNormHeads, p.group - part);
+    for (int g = warp; g < heads; g += kJoinWarps) {
+      const int u = (part + g) / HU;
+      const int2 span = p.span[static_cast<size_t>(bh) * p.units_per_kv + u];
       float2 norm;
       if (span.y < 0) {
-        norm = p.norm[head0 + warp];
+        norm = p.norm[first_head + part + g];
       } else {
-        const float2 ml = joined_ml(p, span.x, span.y, warp, lane);
+        const float2 ml = joined_ml<HU>(p, span.x, span.y, part + g - u * HU, lane);
         norm = weight_norm<T>(ml.x, ml.y);
       }
-      if (lane == 0) head_norm[warp] = norm;
+      if (lane == 0) head_norm[g] = norm;
     }
     __syncthreads();
-    const float *in = u ? out : p.scores + b * p.in_seq + h * p.in_head + k0;
-    constexpr int R = 4;
+    const float *in = part ? out : p.scores + b * p.in_seq + h * p.in_head + k0;
+    const float *logits = p.logits + (first_head + part) * p.logit_row + k0;
+    constexpr int R = 4, H = 8;  // rows and heads of a thread under way at once
     for (int k = tid; k < n; k += R * kJoinThreads) {
-      float x[HU][R], w[R];
-#pragma unroll
-      for (int i = 0; i < R; ++i) w[i] = k + i * kJoinThreads < n ? in[k + i * kJoinThreads] : 0.f;
-#pragma unroll
-      for (int g = 0; g < HU; ++g)
-        if (g < heads) {
-          const float *lg = p.logits + (head0 + g) * p.logit_row + k0 + k;
-#pragma unroll
-          for (int i = 0; i < R; ++i) x[g][i] = k + i * kJoinThreads < n ? lg[i * kJoinThreads] : -INFINITY;
-        }
+      float w[R], sum[R];
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        float sum = 0.f;
+        w[i] = k + i * kJoinThreads < n ? in[k + i * kJoinThreads] : 0.f;
+        sum[i] = 0.f;
+      }
+      for (int g0 = 0; g0 < heads; g0 += H) {
+        float x[H][R];
 #pragma unroll
-        for (int g = 0; g < HU; ++g)
-          if (g < heads) sum = fmaf(fast_exp2(x[g][i] - head_norm[g].x), head_norm[g].y, sum);
-        w[i] += sum;
+        for (int g = 0; g < H; ++g)
+          if (g0 + g < heads) {
+            const float *lg = logits + (g0 + g) * p.logit_row + k;
+#pragma unroll
+            for (int i = 0; i < R; ++i) x[g][i] = k + i * kJoinThreads < n ? lg[i * kJoinThreads] : -INFINITY;
+          }
+#pragma unroll
+        for (int g = 0; g < H; ++g)
+          if (g0 + g < heads) {
+            const float2 norm = head_norm[g0 + g];
+#pragma unroll
+            for (int i = 0; i < R; ++i) sum[i] = fmaf(fast_exp2(x[g][i] - norm.x), norm.y, sum[i]);
+          }
       }
 #pragma unroll
       for (int i = 0; i < R; ++i)
-        if (k + i * kJoinThreads < n) out[k + i * kJoinThreads] = w[i];
+        if (k + i * kJoinThreads < n) out[k + i * kJoinThreads] = w[i] + sum[i];
     }
     __syncthreads();
   }

@@ -212,6 +212,16 @@ def test_attention_heads_and_types(rib, lib, nq, nkv, D, dtype):
     check_attention(rib, lib, [1, 15, 16, 17, 0, 33, 200], nq=nq, nkv=nkv, D=D, page_rows=16, dtype=dtype, scores=True)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("nq,nkv", [(9, 1), (16, 1), (17, 1), (32, 1), (30, 2), (40, 1)])
+def test_attention_more_than_eight_heads_to_a_kv_head(rib, lib, nq, nkv, D, dtype):
+    """Units of 16 query heads, whole, in pieces and in runs, with partly filled units."""
+    check_attention(rib, lib, [1, 17, 0, 250], nq=nq, nkv=nkv, D=D, page_rows=16, dtype=dtype, scores=True)
+    check_attention(rib, lib, [5000, 33, 0, 1200], nq=nq, nkv=nkv, D=D, page_rows=16, dtype=dtype, scores=True, seed=1)
+    check_attention(rib, lib, [40000], nq=nq, nkv=nkv, D=D, page_rows=64, dtype=dtype, scores=nq < 20, seed=2, q_scale=3.0)
+
+
 @pytest.mark.parametrize("page_rows", [16, 32, 48, 64, 256])
 def test_attention_pages_that_end_inside(rib, lib, page_rows):
     check_attention(rib, lib, [page_rows - 1, page_rows, page_rows + 1, 3 * page_rows + 5, 1], nq=4, nkv=2, D=128,
