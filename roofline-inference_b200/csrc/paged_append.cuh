@@ -15,7 +15,7 @@
 // shuffle).  A lane group keeps one token's cosines for all the heads it takes.  A row is short, so what
 // limits the kernel is how many are under way: each lane copies its next heads into a ring of its own
 // (cp.async), 5 ahead.  Measured on B200: 32768 tokens of 16 + 16 heads of 128 dims, normalised, in
-// 91-93 us (5.8 TB/s, 0.89 of the copy rate; loads into registers 119 us); 4093 tokens of 32 + 16 heads,
+// 91-95 us (5.7-5.9 TB/s, 0.86-0.89 of the copy rate; loads into registers 119 us); 4093 tokens of 32 + 16 heads,
 // interleaved over 64 of 128 dims, 20-21 us (4.9 TB/s; with two chunks of neighbouring dims to a lane,
 // half a sector an access, 34 us); one token 2.9 us on the device.
 #pragma once
