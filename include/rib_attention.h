@@ -704,7 +704,9 @@ int rib_paged_append(const rib_paged_cache *cache, const rib_rotary *rot,
  *   nq a multiple of nkv; head_dim 64 or 128; page_rows a multiple of 16;
  *   max_len >= every lens[b], at most width * page_rows.
  * lens[b] == 0 gives a row of zeros.  What pages hold behind a sequence's rows
- * (infinities, NaN) has no effect; an infinite V value within them gives NaN.
+ * (infinities, NaN) has no effect.  Infinite V values within them give
+ * infinities, NaN where both signs meet, NaN gives NaN: every row's weight
+ * counts as positive, however small.
  * With `scores` and `scores_out` (FP32
  * [batch][nkv][>= max_len], rows contiguous; they may be the same buffer):
  *   scores_out[b][h][n] = scores[b][h][n] + the softmax weight of row n

@@ -27,6 +27,7 @@ struct View {
 struct BF16 {
   static __device__ __forceinline__ float2 unpack(uint32_t w) { return make_float2(bf16lo(w), bf16hi(w)); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
+  static constexpr uint32_t kInf = 0x7f80;
   static constexpr int kLift = 0;   // a weight in (0, 1] keeps its relative precision down to 2^-126
 };
 struct F16 {
@@ -34,6 +35,7 @@ struct F16 {
     return __half22float2(*reinterpret_cast<const __half2 *>(&w));
   }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_f16x2(lo, hi); }
+  static constexpr uint32_t kInf = 0x7c00;
   static constexpr int kLift = 14;  // times 2^14, it does down to 2^-28, and below that is off by 2^-39 at most
 };
 

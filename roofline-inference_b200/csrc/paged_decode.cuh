@@ -180,6 +180,45 @@ __device__ __forceinline__ bool next_unit(const DecodeParams &p, Place &c, int u
   return false;
 }
 
+// Which of a lane's dims, dim + 8 i + e at bit 2 i + e for i < S, hold +infinity, -infinity and NaN among the V
+// rows [row, end) of a sequence, 8 of which the warp's lanes of one dim take at a time.
+struct OddDims {
+  uint32_t pos, neg, nan;
+};
+template <class T, int S>
+__device__ __noinline__ OddDims odd_dims(const View &cache, int b, int kvh, int row, int end, int dim) {
+  OddDims x = {0, 0, 0};
+  for (row += (threadIdx.x & 31) >> 2; row < end; row += 8) {
+    const int page = page_of(cache, b, row);
+    if (page < 0) continue;  // counts as zeros
+    const uint16_t *v = cache.pages + page * cache.s_page + cache.s_half + kvh * cache.s_head +
+                        (row % cache.page_rows) * cache.s_row + dim;
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      const uint32_t w = *reinterpret_cast<const uint32_t *>(v + 8 * i);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t u = w >> (16 * e) & 0xffffu, bit = 1u << (2 * i + e);
+        if ((u & 0x7fffu) > T::kInf) x.nan |= bit;
+        if (u == T::kInf) x.pos |= bit;
+        if (u == (T::kInf | 0x8000u)) x.neg |= bit;
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 4; o <= 16; o <<= 1) {
+    x.pos |= __shfl_xor_sync(0xffffffffu, x.pos, o);
+    x.neg |= __shfl_xor_sync(0xffffffffu, x.neg, o);
+    x.nan |= __shfl_xor_sync(0xffffffffu, x.nan, o);
+  }
+  return x;
+}
+// The sum over such a dim, every weight counting as positive; `sum` where there are none.
+__device__ __forceinline__ float odd_sum(const OddDims &x, uint32_t bit, float sum) {
+  if (!((x.pos | x.neg | x.nan) & bit)) return sum;
+  return (x.nan | (x.pos & x.neg)) & bit ? NAN : x.pos & bit ? INFINITY : -INFINITY;
+}
+
 // (maximum, factor) such that exp2(score - maximum) * factor is a row's weight.
 template <class T>
 __device__ __forceinline__ float2 weight_norm(float M, float L) {
@@ -534,6 +573,36 @@ __global__ void __launch_bounds__(NT, DecodeCfg<D>::CTAS) paged_decode_kernel(co
       const bool whole = c.tile == 0 && seg == c.tiles;
       const int part = c.tile > 0 ? 0 : 1;
       const int d0 = warp * (D / NW) + 2 * t4;
+      float2 sum[R][S];
+      bool odd = false;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+          float2 v = make_float2(0.f, 0.f);  // in warp order
+#pragma unroll
+          for (int w = 0; w < NW; ++w) {
+            const float2 u = w == warp ? own[r][i]
+                                       : *reinterpret_cast<const float2 *>(
+                                             &sm.o[warp][w - (w > warp)][g + 8 * r][i * 8 + 2 * t4]);
+            v.x += u.x;
+            v.y += u.y;
+          }
+          sum[r][i] = v;
+          odd |= !(fabsf(v.x) < INFINITY) || !(fabsf(v.y) < INFINITY);
+        }
+      // Infinite and NaN values: the two parts of a weight times an infinity may make NaN of what the weight itself
+      // makes an infinity, so the V rows are asked which dims hold some.
+      if (__any_sync(0xffffffffu, odd)) {
+        const OddDims x = odd_dims<T, S>(p.cache, c.b, kvh, c.tile * TK, min(c.n, (c.tile + seg) * TK), d0);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int i = 0; i < S; ++i) {
+            sum[r][i].x = odd_sum(x, 1u << (2 * i), sum[r][i].x);
+            sum[r][i].y = odd_sum(x, 2u << (2 * i), sum[r][i].y);
+          }
+      }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const int hd = g + 8 * r;
@@ -545,14 +614,7 @@ __global__ void __launch_bounds__(NT, DecodeCfg<D>::CTAS) paged_decode_kernel(co
         float *po = p.part_o + ((static_cast<size_t>(cta) * 2 + part) * HU + hd) * D + d0;
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-          float2 v = make_float2(0.f, 0.f);  // in warp order
-#pragma unroll
-          for (int w = 0; w < NW; ++w) {
-            const float2 u = w == warp ? own[r][i]
-                                       : *reinterpret_cast<const float2 *>(&sm.o[warp][w - (w > warp)][hd][i * 8 + 2 * t4]);
-            v.x += u.x;
-            v.y += u.y;
-          }
+          const float2 v = sum[r][i];
           if (hd < heads) {
             if (whole)
               *reinterpret_cast<uint32_t *>(out + 8 * i) = T::pack(v.x * inv, v.y * inv);
@@ -655,10 +717,14 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
         for (int i = 0; i < N; ++i) {
           if (c0 + i * step > r.last) continue;
           const float al = all.x == -INFINITY ? 0.f : fast_exp2(m[i] - all.x);
-          o.x = fmaf(u[i].x, al, o.x);
-          o.y = fmaf(u[i].y, al, o.y);
-          o.z = fmaf(u[i].z, al, o.z);
-          o.w = fmaf(u[i].w, al, o.w);
+          if (al != 0.f) {
+            o = make_float4(fmaf(u[i].x, al, o.x), fmaf(u[i].y, al, o.y), fmaf(u[i].z, al, o.z), fmaf(u[i].w, al, o.w));
+          } else {  // infinite and NaN values show whatever their weight
+            const float *from = &u[i].x;
+            float *to = &o.x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to[e] += fabsf(from[e]) < INFINITY ? 0.f : from[e];
+          }
         }
       }
       if (R == 2) {

@@ -131,6 +131,8 @@ def paged_decode_attention(q, pages, table, lens, scale: float, *, max_len: int 
     sizes nothing but the scores' scratch.  scores [B, nkv, >= max_len] FP32: the softmax weight of
     each row, summed over the query heads of its KV head, is added to it, in place or into scores_out
     (scores itself, or a buffer that does not overlap it); entries behind lens[b] stay as they are.
+    Infinite V values give infinities, NaN where both signs meet, NaN gives NaN: every row's weight counts
+    as positive, however small.
     Weights and sums are FP32; the result is rounded once."""
     return _lib.binding().paged_decode_attention(q, pages, table, lens, scale, max_len, scores, scores_out, out)
 
