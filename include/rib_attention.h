@@ -645,9 +645,10 @@ int rib_tp_reduce_add_rms(const rib_tp_prefill_exchange *ex, int M,
  * 8; the last dimension is contiguous).  Row r of sequence s lies in page
  * table[s][r / page_rows] at r % page_rows.  A table entry outside
  * [0, num_pages) names no page; entries behind a sequence's rows are never
- * read.  width * page_rows is at most 0x7f000000.  None of the calls keeps
- * state or needs a cleared workspace, so calls on different streams, and
- * captured graphs, are independent as long as each has buffers of its own.
+ * read.  width * page_rows, keep and new_score_rows are at most 0x7f000000.
+ * None of the calls keeps state or needs a cleared workspace, so calls on
+ * different streams, and captured graphs, are independent as long as each has
+ * buffers of its own.
  * Like this library's other kernels they trigger programmatic launch, so
  * their results are not among the rows that rib_decode_attention_qkv may read
  * when it is the very next launch.

@@ -9,6 +9,9 @@
 
 namespace {
 
+// Rows are 32-bit numbers, and a loop over them steps past its end by up to as many rows as it takes at once.
+constexpr long long kMostRows = 0x7f000000;
+
 inline bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 // Strides of 16-byte vectors (16-bit elements).
 template <typename... S>
@@ -22,7 +25,7 @@ int paged_view(const rib_paged_cache *c, rib::paged::View *v) {
       c->head_dim > 256 || c->head_dim % 16 || c->table_stride < 0 || c->stride_page < 0 || c->stride_half < 0 ||
       c->stride_head < 0 || c->stride_row < c->head_dim)
     return RIB_EINVAL;
-  if (static_cast<long long>(c->width) * c->page_rows > 0x7f000000LL) return RIB_EINVAL;  // rows are 32-bit numbers
+  if (static_cast<long long>(c->width) * c->page_rows > kMostRows) return RIB_EINVAL;
   if (!aligned16(c->pages) || !aligned4(c->table) ||
       !strides8(c->stride_page, c->stride_half, c->stride_head, c->stride_row))
     return RIB_EALIGN;
@@ -373,8 +376,9 @@ int rib_paged_evict(const rib_paged_cache *cache, const int32_t *new_table, long
   if (ms != RIB_OK) return ms;
   if (!lens || !scores || !rows || !new_lens || batch < 1 || batch > cache->seqs || batch > 65535 ||
       cache->nkv > 65535 || max_len < 1 || max_len > static_cast<long long>(cache->width) * cache->page_rows ||
-      keep < 1 || sinks < 0 || recent < 0 || static_cast<long long>(sinks) + recent > keep ||
-      std::min(keep, max_len) > static_cast<long long>(new_width) * cache->page_rows || (new_scores && new_score_rows < keep) ||
+      keep < 1 || keep > kMostRows || sinks < 0 || recent < 0 || static_cast<long long>(sinks) + recent > keep ||
+      std::min(keep, max_len) > static_cast<long long>(new_width) * cache->page_rows ||
+      (new_scores && (new_score_rows < keep || new_score_rows > kMostRows)) ||
       (cache->head_dim != 64 && cache->head_dim != 128))
     return RIB_EINVAL;
   if (!aligned4(lens) || !aligned4(scores) || !aligned4(rows) || !aligned4(new_lens) || !aligned4(new_scores))

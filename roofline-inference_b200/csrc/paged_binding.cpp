@@ -34,6 +34,8 @@ decltype(&rib_paged_decode_workspace_bytes) decode_workspace_bytes;
 decltype(&rib_paged_decode_attention) decode_attention_fn;
 decltype(&rib_paged_evict) paged_evict_fn;
 
+constexpr int kMostRows = 0x7f000000;  // as the library has it
+
 struct Refused {};  // a Python exception is set
 
 [[noreturn]] void refuse(const char *fmt, ...) {
@@ -352,6 +354,7 @@ PyObject *paged_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const int keep = number(a[4], "keep"), sinks = number(a[6], "sinks"), recent = number(a[7], "recent");
     if (keep < 1 || sinks < 0 || recent < 0 || static_cast<int64_t>(sinks) + recent > keep)
       refuse("need keep >= 1, sinks >= 0, recent >= 0 and sinks + recent <= keep");
+    if (keep > kMostRows) refuse("keep must be at most %d", kMostRows);
     const int most = std::min(keep, max_len);
     if (table.size(0) < batch || table.size(1) * cache.page_rows < most)
       refuse("new_table must name pages for %d rows of %d sequences, got %s", most, batch, shape_of(table).c_str());
@@ -364,7 +367,8 @@ PyObject *paged_evict(PyObject *, PyObject *const *a, Py_ssize_t n) {
       if (x.first < y.second && y.first < x.second) refuse("new_scores must not overlap scores");
       kept = written(t, "new_scores").data_ptr<float>();
       kept_s[0] = step(t, 0), kept_s[1] = step(t, 1);
-      kept_rows = size32(t.size(2), "new_scores");
+      if (t.size(2) > kMostRows) refuse("new_scores must have at most %d entries a head", kMostRows);
+      kept_rows = static_cast<int>(t.size(2));
     }
     const c10::cuda::CUDAGuard guard(dev);
     const at::Tensor rows = fresh({batch, cache.nkv, keep}, at::kInt, dev), new_lens = fresh({batch}, at::kInt, dev);

@@ -149,5 +149,5 @@ def paged_evict(pages, table, lens, scores, keep: int, new_table, *, sinks: int 
     left as they were.  rows [B, nkv, keep] int32: the old row of each new one, -1 behind the last;
     new_lens [B] int32.  new_scores [B, nkv, >= keep]: receives the kept rows' scores and zeros behind
     them.  Heads of one sequence keep different rows, so positions must be those the keys were rotated
-    with: a row number is not one any more."""
+    with: a row number is not one any more.  keep may exceed what any sequence has, up to 0x7f000000."""
     return _lib.binding().paged_evict(pages, table, lens, scores, keep, new_table, sinks, recent, max_len, new_scores)

@@ -93,3 +93,15 @@ def test_attention_infinite_and_nan_values(rib, lib, low, n, nq, nkv, D, dtype):
     rest = torch.tensor([d for d in range(D) if d not in (1, 2, 3, 4, 5, D - 1)], device="cuda")
     a, w, b = got[..., rest].double(), want[..., rest], bound[..., rest]
     assert ((a - w).abs() <= w.abs() * half_step(dtype) + smallest_half(dtype) + b).all()
+
+
+# ------------------------------------------------------------------ eviction
+def test_evict_keep_is_bounded(rib, lib):
+    """`keep` beyond what the loops over rows count to is refused on the host, before its buffers are made."""
+    pages, table = make_cache([40], 1, 64, 16, BF16, gen(0), fill=0.0)
+    scores = torch.rand((1, 1, 48), generator=gen(1)).cuda()
+    before = pages.clone()
+    for keep in (0x7f000001, 2 ** 31 - 1):
+        with pytest.raises(ValueError, match="keep"):
+            rib.paged_evict(pages, table, i32([40]), scores, keep, table)
+    assert torch.equal(pages, before) and lib.take_device_status() == 0

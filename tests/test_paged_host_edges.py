@@ -1,0 +1,21 @@
+"""CPU: paged-cache calls at the edges of what they take, and the page accounting of PagedDecoder.  No call here
+reaches a kernel launch."""
+from __future__ import annotations
+
+import pytest
+
+from test_paged_host import EINVAL, FAKE, cache
+
+MOST = 0x7f000000
+
+
+@pytest.mark.parametrize("keep,new_rows", [(MOST + 1, MOST + 1), (2 ** 31 - 1, 2 ** 31 - 1), (32, MOST + 1),
+                                           (32, 2 ** 31 - 1)])
+def test_evict_refuses_more_rows_than_its_loops_count(rib, keep, new_rows):
+    """A thread of the selection writes every 512th to 8192nd of `keep` rows (and of the score rows behind them),
+    counting in 32 bits: for a keep within that many of 2^31 the count would wrap and the thread write far below its
+    buffer.  Refused before anything is launched."""
+    L = rib.load_library()
+    status = L.rib_paged_evict(cache(), FAKE, 2, 2, FAKE, 3, 32, FAKE, 128, 64, keep, 4, 8, FAKE, FAKE, FAKE, 64, 32,
+                               new_rows, None)
+    assert status == EINVAL
