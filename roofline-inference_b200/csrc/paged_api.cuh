@@ -321,6 +321,10 @@ int rib_paged_decode_attention(const rib_paged_cache *cache, const void *q, long
       (dim != 64 && dim != 128) || cache->page_rows % TK || !scores != !scores_out)
     return RIB_EINVAL;
   const PagedDecodeLayout l = paged_decode_layout(batch, max_len, nq, dim, scores != nullptr);
+  const int group = nq / cache->nkv, units_per_kv = ceil_div(group, unit_heads(group));
+  // a CTA counts the tiles of its run in 32 bits
+  if (static_cast<double>(batch) * cache->nkv * units_per_kv * ceil_div(max_len, TK) > static_cast<double>(kMostRows) * l.grid)
+    return RIB_EINVAL;
   if (!workspace || workspace_bytes < l.total) return RIB_EINVAL;
   if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || !aligned4(lens) || !aligned4(scores) ||
       !aligned4(scores_out) || !strides8(q_seq, q_head))
@@ -335,8 +339,8 @@ int rib_paged_decode_attention(const rib_paged_cache *cache, const void *q, long
   p.lens = lens;
   p.batch = batch;
   p.nq = nq;
-  p.group = nq / cache->nkv;
-  p.units_per_kv = ceil_div(p.group, unit_heads(p.group));
+  p.group = group;
+  p.units_per_kv = units_per_kv;
   p.max_len = max_len;
   p.scale2 = static_cast<float>(scale * 1.4426950408889634);
   p.whole = max_len <= kWholeRows;

@@ -19,3 +19,14 @@ def test_evict_refuses_more_rows_than_its_loops_count(rib, keep, new_rows):
     status = L.rib_paged_evict(cache(), FAKE, 2, 2, FAKE, 3, 32, FAKE, 128, 64, keep, 4, 8, FAKE, FAKE, FAKE, 64, 32,
                                new_rows, None)
     assert status == EINVAL
+
+
+def test_attention_refuses_more_tiles_than_a_run_counts(rib):
+    """A CTA counts the tiles of its run in 32 bits. Sequences that share their pages (a table stride of 0) can add up
+    to more than the 148 x 2 or x 3 CTAs count: the run's length would wrap, and the join would read records that
+    nothing wrote."""
+    L = rib.load_library()
+    many = cache(seqs=1 << 20, nkv=1 << 10, width=MOST // 256, page_rows=256, table_stride=0)
+    status = L.rib_paged_decode_attention(many, FAKE, 1 << 16, 64, FAKE, 1 << 20, 1 << 10, MOST, 0.125, FAKE, None, 0, 0,
+                                          None, 0, 0, FAKE, 1 << 40, None)
+    assert status == EINVAL
