@@ -317,7 +317,8 @@ int rib_paged_decode_attention(const rib_paged_cache *cache, const void *q, long
   if (cs != RIB_OK) return cs;
   const int dim = cache->head_dim;
   if (!q || !lens || !out || batch < 1 || batch > cache->seqs || nq < 1 || nq % cache->nkv || max_len < 1 ||
-      max_len > static_cast<long long>(cache->width) * cache->page_rows || !(scale > 0.f) || !(scale < INFINITY) ||
+      max_len > static_cast<long long>(cache->width) * cache->page_rows || !(scale > 0.f) ||
+      !(scale * 1.4426950408889634 < 3.4e38) ||  // scores are formed in log2 units
       (dim != 64 && dim != 128) || cache->page_rows % TK || !scores != !scores_out)
     return RIB_EINVAL;
   const PagedDecodeLayout l = paged_decode_layout(batch, max_len, nq, dim, scores != nullptr);

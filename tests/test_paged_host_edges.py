@@ -30,3 +30,12 @@ def test_attention_refuses_more_tiles_than_a_run_counts(rib):
     status = L.rib_paged_decode_attention(many, FAKE, 1 << 16, 64, FAKE, 1 << 20, 1 << 10, MOST, 0.125, FAKE, None, 0, 0,
                                           None, 0, 0, FAKE, 1 << 40, None)
     assert status == EINVAL
+
+
+def test_attention_refuses_a_scale_beyond_fp32_in_log2_units(rib):
+    """scale * log2 e has to be finite in FP32: beyond it a score of 0 would be 0 times infinity."""
+    L = rib.load_library()
+    ws = L.rib_paged_decode_workspace_bytes(3, 64, 4, 64, 0)
+    for scale in (2.4e38, 3.4e38):
+        assert L.rib_paged_decode_attention(cache(), FAKE, 256, 64, FAKE, 3, 4, 64, scale, FAKE, None, 0, 0, None, 0, 0,
+                                            FAKE, ws, None) == EINVAL
