@@ -233,11 +233,18 @@ class PagedDecoder:
         if full and self.keep is None:
             raise ValueError("KV capacity exceeded")
         P = self.pool.page_rows
-        # an eviction takes its new pages before it gives the old ones back: one sequence at a time
         growing = [i for i in live if i not in full and self.rows[i] == len(self.pages[i]) * P]
-        short = self.pool.pages_for(self.keep) if full else 0
-        if len(growing) + short > self.pool.free_pages:
-            raise PoolFull(f"{len(growing) + short} pages wanted, {self.pool.free_pages} free")
+        # what the loops below take and give, in their order: an eviction takes its new pages before it gives the
+        # old ones back, which the next eviction, and then the growing sequences, can use
+        free = self.pool.free_pages
+        wants = self.pool.pages_for(self.keep) if full else 0
+        for i in full:
+            if wants > free:
+                raise PoolFull(f"{wants} pages wanted for an eviction, {free} free")
+            free += len(self.pages[i]) - wants
+        grow = len(growing) + (len(full) if full and self.keep == wants * P else 0)
+        if grow > free:
+            raise PoolFull(f"{grow} pages wanted, {free} free")
         for i in full:
             self._evict(i)
             if self.keep == len(self.pages[i]) * P:

@@ -2,7 +2,11 @@
 reaches a kernel launch."""
 from __future__ import annotations
 
+import importlib
+from types import SimpleNamespace
+
 import pytest
+import torch
 
 from test_paged_host import EINVAL, FAKE, cache
 
@@ -39,3 +43,62 @@ def test_attention_refuses_a_scale_beyond_fp32_in_log2_units(rib):
     for scale in (2.4e38, 3.4e38):
         assert L.rib_paged_decode_attention(cache(), FAKE, 256, 64, FAKE, 3, 4, 64, scale, FAKE, None, 0, 0, None, 0, 0,
                                             FAKE, ws, None) == EINVAL
+
+
+# ------------------------------------------------------------------ PagedDecoder's pages
+def decoder(rib, rows, *, pages, max_rows, keep=None, layers=2, page_rows=16):
+    """A decoder with one sequence of rows[i] rows in slot i, whose device work is stubbed out by the caller."""
+    engine = SimpleNamespace(world=1, cfg=SimpleNamespace(num_layers=layers), device=torch.device("cpu"), n_kv=1,
+                             nq_local=2, base=1e6, layers=[{}] * layers)
+    pool = rib.PagePool(layers, 1, pages, page_rows, device="cpu")
+    d = rib.PagedDecoder(engine, pool, len(rows), max_rows, keep=keep, sinks=0, recent=0)
+    for i, n in enumerate(rows):
+        ids = pool.take(pool.pages_for(n))
+        d.pages[i] = ids
+        d.table[i, :len(ids)] = torch.tensor(ids, dtype=torch.int32)
+        d._set_rows(i, n)
+    return d, pool
+
+
+def pages_of(d):
+    return (list(d.rows), [list(p) for p in d.pages], d.row.tolist(), d.lens.tolist(), d.table.tolist(),
+            d.pool.free_pages)
+
+
+@pytest.fixture
+def no_eviction(monkeypatch):
+    """paged_evict without its device work."""
+    module = importlib.import_module("roofline-inference_b200.paged_batch")
+    calls = []
+    monkeypatch.setattr(module, "paged_evict", lambda *a, **kw: calls.append(a))
+    return calls
+
+
+@pytest.mark.parametrize("rows,pages,max_rows,keep,after", [
+    ([64, 16], 6, 64, 16, [2, 2]),           # 1 free: the eviction gives 4 back, then both grow
+    ([64, 64, 16], 10, 64, 16, [2, 2, 2]),   # 1 free: the second eviction lives on the first one's pages
+    ([64, 48], 9, 64, 20, [2, 4]),           # 2 free, both for the eviction, which leaves room for the other
+    ([17, 16], 4, 17, 16, [2, 2]),           # every page in use afterwards
+])
+def test_eviction_frees_the_pages_that_others_grow_into(rib, no_eviction, rows, pages, max_rows, keep, after):
+    d, pool = decoder(rib, rows, pages=pages, max_rows=max_rows, keep=keep)
+    d._make_room()
+    assert [len(p) for p in d.pages] == after
+    assert d.rows == [keep if n == max_rows else n for n in rows]
+    used = [p for ids in d.pages for p in ids]
+    assert len(set(used)) == len(used) and pool.free_pages == len(pool.layer(0)) - len(used)
+    for i, ids in enumerate(d.pages):
+        assert d.table[i].tolist() == ids + [-1] * (d.table.shape[1] - len(ids))
+
+
+@pytest.mark.parametrize("rows,pages,max_rows,keep", [
+    ([64, 16], 6, 64, 32),            # an eviction to 2 pages with 1 free
+    ([64], 4, 64, 16),                # ... to 1 page with none
+    ([17, 16, 16], 5, 17, 16),        # the eviction fits, the three that grow afterwards do not
+])
+def test_room_that_is_not_there_changes_nothing(rib, no_eviction, rows, pages, max_rows, keep):
+    d, _ = decoder(rib, rows, pages=pages, max_rows=max_rows, keep=keep)
+    before = pages_of(d)
+    with pytest.raises(rib.PoolFull):
+        d._make_room()
+    assert pages_of(d) == before and not no_eviction
