@@ -106,7 +106,7 @@ class PagedDecoder:
         if keep is not None:
             room = width * pool.page_rows
             self.scores = torch.zeros((cfg.num_layers, slots, engine.n_kv, room), device=dev)
-            self._kept = torch.empty((1, engine.n_kv, room), device=dev)
+            self._kept = torch.empty((cfg.num_layers, 1, engine.n_kv, room), device=dev)
         self.pages: list[list[int] | None] = [None] * slots   # host side: each slot's pages,
         self.rows = [0] * slots                                 # rows,
         self.positions = [0] * slots                            # and next position
@@ -129,11 +129,11 @@ class PagedDecoder:
             raise ValueError("KV capacity exceeded")
         i, ids = free[0], self.pool.take(self.pool.pages_for(n))
         try:
-            logits = self._prefill(torch.tensor(prompt, dtype=torch.int32, device=self.device), ids)
+            first = argmax(self._prefill(torch.tensor(prompt, dtype=torch.int32, device=self.device), ids))
         except BaseException:
             self.pool.give(ids)
             raise
-        self.tok[i:i + 1].copy_(argmax(logits))
+        self.tok[i:i + 1].copy_(first)
         self.pages[i], self.rows[i], self.positions[i] = ids, n, n
         self.table[i].fill_(-1)
         self.table[i, :len(ids)] = torch.tensor(ids, dtype=torch.int32).to(self.device)
@@ -259,11 +259,14 @@ class PagedDecoder:
         new = torch.full_like(self.table[i:i + 1], -1)
         new[0, :len(ids)] = torch.tensor(ids, dtype=torch.int32).to(self.device)
         lens = self.row[i:i + 1]  # rows in the cache: the next token's row
-        for l in range(len(self.e.layers)):
-            scores = self.scores[l, i:i + 1]
-            paged_evict(self.pool.layer(l), self.table[i:i + 1], lens, scores, self.keep, new, sinks=self.sinks,
-                        recent=self.recent, new_scores=self._kept)
-            scores.copy_(self._kept)
+        try:
+            for l in range(len(self.e.layers)):
+                paged_evict(self.pool.layer(l), self.table[i:i + 1], lens, self.scores[l, i:i + 1], self.keep, new,
+                            sinks=self.sinks, recent=self.recent, new_scores=self._kept[l])
+        except BaseException:  # the sequence is as it was: its own pages and scores were only read
+            self.pool.give(ids)
+            raise
+        self.scores[:, i:i + 1].copy_(self._kept)
         self.table[i:i + 1].copy_(new)
         self.pool.give(self.pages[i])
         self.pages[i] = ids

@@ -102,3 +102,35 @@ def test_room_that_is_not_there_changes_nothing(rib, no_eviction, rows, pages, m
     with pytest.raises(rib.PoolFull):
         d._make_room()
     assert pages_of(d) == before and not no_eviction
+
+
+def test_eviction_that_fails_leaves_the_sequence_as_it_was(rib, monkeypatch):
+    """A layer's eviction that raises (memory for its outputs, say): pages, rows and all layers' scores stay."""
+    module = importlib.import_module("roofline-inference_b200.paged_batch")
+    d, pool = decoder(rib, [64], pages=6, max_rows=64, keep=16, layers=3)
+    d.scores.copy_(torch.rand(d.scores.shape))
+    before, scores = pages_of(d), d.scores.clone()
+
+    def fails_in_layer_1(pages, *a, new_scores, **kw):
+        if pages.data_ptr() == pool.layer(1).data_ptr():
+            raise RuntimeError("out of memory")
+        new_scores.fill_(7.0)
+    monkeypatch.setattr(module, "paged_evict", fails_in_layer_1)
+    with pytest.raises(RuntimeError, match="out of memory"):
+        d._make_room()
+    assert pages_of(d) == before and torch.equal(d.scores, scores)
+
+
+def test_add_that_fails_gives_its_pages_back(rib, monkeypatch):
+    module = importlib.import_module("roofline-inference_b200.paged_batch")
+    d, pool = decoder(rib, [16], pages=6, max_rows=64)
+    d.remove(0)
+    d.e.cfg.vocab_size = 10
+    monkeypatch.setattr(rib.PagedDecoder, "_prefill", lambda self, tokens, ids: None)
+
+    def fails(logits):
+        raise RuntimeError("out of memory")
+    monkeypatch.setattr(module, "argmax", fails)
+    with pytest.raises(RuntimeError, match="out of memory"):
+        d.add([1, 2, 3])
+    assert pool.free_pages == 6 and d.free_slots() == [0]
