@@ -2,7 +2,7 @@
 binding of its paged-cache entry points (_paged_binding.so).
 
 The library is built in-tree from csrc/ with nvcc.  `load()` rebuilds it when
-the sources changed (content hash, not mtimes, so a copied tree is recognised
+its sources changed (content hash, not mtimes, so a copied tree is recognised
 correctly) and then binds the entry points declared in
 include/rib_attention.h with ctypes.  There is no fallback: if the library
 cannot be built or loaded, every call raises.
@@ -100,34 +100,50 @@ def binding_is_current() -> bool:
     return BINDING_PATH.exists() and BINDING_STAMP.exists() and BINDING_STAMP.read_text().strip() == binding_hash()
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compiles csrc/rib_attention.cu for sm_100a into librib_attention.so, and
-    csrc/paged_binding.cpp against this process's torch into _paged_binding.so.
-
-    Serialised with a file lock so that several ranks importing the package at
-    once build them only once."""
-    if not force and is_current() and binding_is_current():
-        return LIB_PATH
-    lock_path = PKG_DIR / ".librib_attention.lock"
-    with open(lock_path, "w") as lock:
+def _build_locked(current, make, force: bool) -> None:
+    """Runs `make` unless `current()`.  Serialised with a file lock so that several ranks importing the
+    package at once build only once."""
+    if not force and current():
+        return
+    with open(PKG_DIR / ".librib_attention.lock", "w") as lock:
         fcntl.flock(lock, fcntl.LOCK_EX)
         try:
-            if force or not is_current():
-                tmp = LIB_PATH.with_name(f"{LIB_PATH.name}.{os.getpid()}.tmp")
-                cmd = [_nvcc(), *NVCC_FLAGS, "-o", str(tmp), str(MAIN_SOURCE)]
-                if verbose:
-                    cmd.insert(1, "-Xptxas=-v")
-                _run(cmd, "nvcc", verbose)
-                tmp.replace(LIB_PATH)
-                STAMP.write_text(source_hash() + "\n")
-            if force or not binding_is_current():
-                tmp = BINDING_PATH.with_name(f"{BINDING_PATH.name}.{os.getpid()}.tmp")
-                _run([*_binding_command(), "-o", str(tmp)], "g++", verbose)
-                tmp.replace(BINDING_PATH)
-                BINDING_STAMP.write_text(binding_hash() + "\n")
+            if force or not current():
+                make()
         finally:
             fcntl.flock(lock, fcntl.LOCK_UN)
+
+
+def build_library(force: bool = False, verbose: bool = False) -> Path:
+    """Compiles csrc/rib_attention.cu for sm_100a into librib_attention.so."""
+    def make():
+        tmp = LIB_PATH.with_name(f"{LIB_PATH.name}.{os.getpid()}.tmp")
+        cmd = [_nvcc(), *NVCC_FLAGS, "-o", str(tmp), str(MAIN_SOURCE)]
+        if verbose:
+            cmd.insert(1, "-Xptxas=-v")
+        _run(cmd, "nvcc", verbose)
+        tmp.replace(LIB_PATH)
+        STAMP.write_text(source_hash() + "\n")
+    _build_locked(is_current, make, force)
     return LIB_PATH
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> Path:
+    """Compiles csrc/paged_binding.cpp against this process's torch into _paged_binding.so."""
+    def make():
+        tmp = BINDING_PATH.with_name(f"{BINDING_PATH.name}.{os.getpid()}.tmp")
+        _run([*_binding_command(), "-o", str(tmp)], "g++", verbose)
+        tmp.replace(BINDING_PATH)
+        BINDING_STAMP.write_text(binding_hash() + "\n")
+    _build_locked(binding_is_current, make, force)
+    return BINDING_PATH
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    """Compiles the library and the binding where their sources changed (or `force`)."""
+    path = build_library(force, verbose)
+    build_binding(force, verbose)
+    return path
 
 
 def _bind(L: ctypes.CDLL) -> None:
@@ -181,10 +197,11 @@ def _bind(L: ctypes.CDLL) -> None:
 
 
 def load() -> ctypes.CDLL:
-    """Builds if needed, loads and binds the library (once per process)."""
+    """Builds if needed, loads and binds the library (once per process).  The Python binding of the paged-cache
+    calls is left to binding(): a library that is up to date needs no compiler."""
     global _lib
     if _lib is None:
-        path = build()
+        path = build_library()
         L = ctypes.CDLL(str(path))
         _bind(L)
         _lib = L
@@ -192,10 +209,11 @@ def load() -> ctypes.CDLL:
 
 
 def binding():
-    """The native binding of the paged-cache entry points (once per process)."""
+    """The native binding of the paged-cache entry points, built if needed (once per process)."""
     global _binding_module
     if _binding_module is None:
         L = load()
+        build_binding()
         spec = importlib.util.spec_from_file_location("_paged_binding", BINDING_PATH)
         m = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(m)

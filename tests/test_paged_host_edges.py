@@ -134,3 +134,22 @@ def test_add_that_fails_gives_its_pages_back(rib, monkeypatch):
     with pytest.raises(RuntimeError, match="out of memory"):
         d.add([1, 2, 3])
     assert pool.free_pages == 6 and d.free_slots() == [0]
+
+
+# ------------------------------------------------------------------ building
+def test_library_loads_without_a_host_compiler(rib, monkeypatch):
+    """A library that is up to date loads whatever became of the binding (another torch, no g++); only the calls
+    that need the binding ask for it, and fail loudly."""
+    L = importlib.import_module("roofline-inference_b200._lib")
+    L.load()
+
+    def no_compiler(*a):
+        raise RuntimeError("no compiler")
+    monkeypatch.setattr(L, "_lib", None)
+    monkeypatch.setattr(L, "_binding_module", None)
+    monkeypatch.setattr(L, "binding_is_current", lambda: False)
+    monkeypatch.setattr(L, "_run", no_compiler)
+    monkeypatch.setattr(L, "_nvcc", no_compiler)
+    assert L.load().rib_version() > 0
+    with pytest.raises(RuntimeError, match="no compiler"):
+        L.binding()
