@@ -302,7 +302,7 @@ class PagedDecoder:
 
     def step(self) -> torch.Tensor:
         """One step of every active slot on the tokens in `tok`; returns the next greedy tokens (int32
-        [slots], which also become the next inputs; idle slots' entries are meaningless)."""
+        [slots], the caller's own, which also become the next inputs; idle slots' entries are meaningless)."""
         self._make_room()
         if self.graph is None:
             self._argmax(self._forward())
@@ -310,7 +310,7 @@ class PagedDecoder:
         else:
             self.graph.replay()
         self._advance_host()
-        return self.next
+        return self.next.clone()
 
     def logits(self) -> torch.Tensor:
         """One eager step; returns the FP32 logits [slots, vocab] and leaves `tok` alone."""

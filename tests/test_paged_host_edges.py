@@ -153,3 +153,19 @@ def test_library_loads_without_a_host_compiler(rib, monkeypatch):
     assert L.load().rib_version() > 0
     with pytest.raises(RuntimeError, match="no compiler"):
         L.binding()
+
+
+def test_step_returns_a_tensor_of_the_callers_own(rib, monkeypatch):
+    """What a step returned stays what it was when later steps run, eager or replayed."""
+    d, _ = decoder(rib, [3], pages=6, max_rows=64)
+    monkeypatch.setattr(rib.PagedDecoder, "_forward", lambda self: None)
+    monkeypatch.setattr(rib.PagedDecoder, "_argmax", lambda self, logits: self.next.copy_(self.tok + 1))
+    d.tok.fill_(5)
+    first = d.step()
+    second = d.step()
+    assert (first.tolist(), second.tolist(), d.tok.tolist()) == ([6], [7], [7])
+    d.graph = SimpleNamespace(replay=lambda: (d.next.fill_(40), d.tok.copy_(d.next)))
+    third = d.step()
+    d.graph = SimpleNamespace(replay=lambda: (d.next.fill_(41), d.tok.copy_(d.next)))
+    d.step()
+    assert (first.tolist(), second.tolist(), third.tolist()) == ([6], [7], [40])
