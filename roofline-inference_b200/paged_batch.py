@@ -18,6 +18,7 @@ from . import _lib
 from ._tensors import HEAD_DIM, stream_handle
 from .attention import attention
 from .batch import _linear as _linear_rows
+from .cache import Cache
 from .kernels import add_rms, argmax, embedding, gemv, rms_norm
 from .model import _linear
 from .paged import Rotary, paged_append, paged_decode_attention, paged_evict
@@ -163,10 +164,11 @@ class PagedDecoder:
 
     # ---------------------------------------------------------------- prefill
     def _prefill(self, tokens, ids: list[int]):
-        """The prompt's forward over a contiguous scratch cache, which is one large page to the append;
-        its rows then go to the sequence's pages.  Returns the FP32 logits of the last row."""
+        """The prompt's forward over one layer's contiguous scratch cache, which is one large page to the append and
+        serves every layer in turn: its rows go to the sequence's pages before the next layer's overwrite them.
+        Returns the FP32 logits of the last row."""
         e, n, P = self.e, tokens.numel(), self.pool.page_rows
-        cache = e.new_cache(n)
+        kv = Cache(1, e.n_kv, HEAD_DIM, n, device=self.device).kv[0]
         pos = torch.arange(n, dtype=torch.int32, device=self.device)
         seq = torch.zeros_like(pos)
         one_page = torch.zeros((1, 1), dtype=torch.int32, device=self.device)
@@ -175,7 +177,6 @@ class PagedDecoder:
         h = embedding(e.embed, tokens)
         x = rms_norm(h, e.layers[0]["in_norm"])
         for l, w in enumerate(e.layers):
-            kv = cache.kv[l]
             self._append(_linear(x, w["qkv"]), w, pos, pos, kv[None], one_page, seq, q.transpose(0, 1)[:n])
             self.pool.layer(l)[where] = kv.view(2, e.n_kv, -1, P, HEAD_DIM)[:, :, :len(ids)].permute(2, 0, 1, 3, 4)
             o = attention(q, kv[0], kv[1], n, n, e.scale)
