@@ -64,7 +64,8 @@ def rotary_frequencies(rotary_dim: int, base: float, scaling: str | None = None,
     # the pair that turns t times over original_length
     pair = [r * math.log(original_length / (t * 2 * math.pi)) / (2 * math.log(base)) for t in (fast_turns, slow_turns)]
     low, high = max(math.floor(pair[0]), 0), min(math.ceil(pair[1]), r - 1)
-    ramp = [min(1.0, max(0.0, (i - low) / max(high - low, 1e-3))) for i in range(r // 2)]
+    # (high <= 0: even pair 0 turns less than slow_turns times)
+    ramp = [1.0 if high <= 0 else min(1.0, max(0.0, (i - low) / max(high - low, 1e-3))) for i in range(r // 2)]
     return [f * (1 - s) + f / factor * s for f, s in zip(freq, ramp)], 1.0 + 0.1 * math.log(factor)
 
 

@@ -3,6 +3,7 @@ reaches a kernel launch."""
 from __future__ import annotations
 
 import importlib
+import math
 from types import SimpleNamespace
 
 import pytest
@@ -169,3 +170,15 @@ def test_step_returns_a_tensor_of_the_callers_own(rib, monkeypatch):
     d.graph = SimpleNamespace(replay=lambda: (d.next.fill_(41), d.tok.copy_(d.next)))
     d.step()
     assert (first.tolist(), second.tolist(), third.tolist()) == ([6], [7], [40])
+
+
+# ------------------------------------------------------------------ frequencies
+@pytest.mark.parametrize("length,slow", [(1, 1.0), (3, 1.0), (6, 1.0), (100, 20.0)])
+def test_yarn_stretches_every_pair_of_a_short_original_length(rib, length, slow):
+    """Pairs that turn less than slow_turns times over original_length are `factor` times slower: all of them where
+    even the fastest (one radian a position) does."""
+    paged = importlib.import_module("roofline-inference_b200.paged")
+    f, _ = paged.rotary_frequencies(64, 1e4)
+    g, _ = paged.rotary_frequencies(64, 1e4, "yarn", 4.0, length, slow_turns=slow)
+    assert length < 2 * math.pi * slow
+    assert g == [x / 4 for x in f]
