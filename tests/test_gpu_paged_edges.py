@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from paged_ref import attend64, half_step, make_cache, smallest_half
+from test_gpu_paged import check_attention
 
 pytestmark = pytest.mark.gpu
 BF16, FP16 = torch.bfloat16, torch.float16
@@ -105,3 +106,92 @@ def test_evict_keep_is_bounded(rib, lib):
         with pytest.raises(ValueError, match="keep"):
             rib.paged_evict(pages, table, i32([40]), scores, keep, table)
     assert torch.equal(pages, before) and lib.take_device_status() == 0
+
+
+# ------------------------------------------------------------------ layouts
+def strided(sizes, order, pad):
+    """Zeros of `sizes` whose dims lie in memory in `order` (outermost first; the last dim innermost), with `pad`
+    elements behind every run of the innermost dims."""
+    strides, step = [0] * len(sizes), 1
+    for d in reversed([*order, len(sizes) - 1]):
+        strides[d] = step
+        step = step * sizes[d] + pad
+    return torch.zeros(step, dtype=BF16, device="cuda").as_strided(sizes, strides)
+
+
+@pytest.mark.parametrize("order,pad", [
+    ((0, 1, 2, 3), 8),    # padded rows, heads, halves and pages: no stride is a multiple of another
+    ((0, 1, 3, 2), 0),    # rows before heads
+    ((1, 0, 2, 3), 0),    # K and V as outer halves
+    ((0, 3, 1, 2), 0),    # a row's K and V together
+    ((2, 0, 1, 3), 0),    # a pool for each head
+    ((3, 2, 1, 0), 24),   # everything the other way round
+])
+@pytest.mark.parametrize("D", [64, 128])
+def test_pages_in_any_order(rib, lib, order, pad, D):
+    """Append, attention and eviction give the same bits whatever the order of the pages' dims in memory."""
+    g = gen(31)
+    nq, nkv, P, lens = 6, 3, 32, [70, 33, 0, 2000]
+    base, table = make_cache(lens, nkv, D, P, BF16, g, spare=40, fill=0.0)
+    free = sorted(set(range(base.shape[0])) - set(table.flatten().tolist()))
+    new = i32([free[:2], free[2:4], [-1, -1], free[4:6]])
+    q, k, v = (torch.randn((4, h, D), generator=g).to(BF16).cuda() for h in (nq, nkv, nkv))
+    scores = torch.rand((4, nkv, table.shape[1] * P), generator=g).cuda()
+    rot, row = rib.Rotary(D), i32([69, 32, -1, 1999])
+    results = []
+    for pages in (base.clone(), strided(base.shape, order, pad)):
+        pages.copy_(base)
+        sc = scores.clone()
+        qr = rib.paged_append(q, k, v, i32([7, 8, 9, 10]), row, pages, table, rot)
+        out = rib.paged_decode_attention(qr, pages, table, i32(lens), 0.1, scores=sc)
+        rows, n = rib.paged_evict(pages, table, i32(lens), sc, 64, new, sinks=3, recent=9)
+        results.append((qr, out, sc, rows, n, pages))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    assert lib.take_device_status() == 0
+    want, _, bound, _ = attend64(results[0][0][:2], base_after_append(base, results[0][5], table, lens), table, lens[:2], 0.1)
+    got = results[1][1][:2]
+    assert ((got.double() - want).abs() <= want.abs() * half_step(BF16) + smallest_half(BF16) + bound).all()
+
+
+def base_after_append(before, after, table, lens):
+    """The pages as the attention saw them: those of the table, before the eviction wrote to others."""
+    pages = before.clone()
+    used = table[table >= 0].long()
+    pages[used] = after[used]
+    return pages
+
+
+def test_append_of_broadcast_heads(rib, lib):
+    """k and v as one head expanded over all KV heads, one token expanded over all sequences."""
+    g = gen(32)
+    nkv, D = 4, 64
+    q = torch.randn((3, 8, D), generator=g).to(BF16).cuda()
+    k = torch.randn((3, 1, D), generator=g).to(BF16).cuda().expand(3, nkv, D)
+    v = torch.randn((1, nkv, D), generator=g).to(BF16).cuda().expand(3, nkv, D)
+    table, rot, pos, row = i32([[0], [1], [2]]), rib.Rotary(D), i32([5, 6, 7]), i32([0, 3, 15])
+    pages = [torch.zeros((3, 2, nkv, 16, D), dtype=BF16, device="cuda") for _ in range(2)]
+    a = rib.paged_append(q, k, v, pos, row, pages[0], table, rot)
+    b = rib.paged_append(q, k.contiguous(), v.contiguous(), pos, row, pages[1], table, rot)
+    assert torch.equal(a, b) and torch.equal(*pages) and (pages[0][1, 1, :, 3] == v[1]).all()
+    before = pages[0].clone()
+    none = rib.paged_append(q[:0], k[:0], v[:0], pos[:0], row[:0], pages[0], table, rot)
+    assert none.shape == (0, 8, D) and torch.equal(pages[0], before)
+    assert lib.take_device_status() == 0
+
+
+# ------------------------------------------------------------------ many heads, bounds on lengths
+@pytest.mark.parametrize("dtype,D", [(BF16, 64), (FP16, 128)])
+@pytest.mark.parametrize("nq,nkv", [(128, 1), (129, 1), (272, 1), (290, 2)])
+def test_attention_row_weights_of_many_heads(rib, lib, nq, nkv, D, dtype):
+    """More than 128 query heads to a KV head: their weights of a row are summed in several passes, of whole and of
+    joined units."""
+    check_attention(rib, lib, [1, 17, 0, 250], nq=nq, nkv=nkv, D=D, page_rows=16, dtype=dtype, scores=True)
+    check_attention(rib, lib, [5000, 33, 0, 1200], nq=nq, nkv=nkv, D=D, page_rows=16, dtype=dtype, scores=True, seed=1)
+
+
+@pytest.mark.parametrize("max_len", [200, 256, 257, 1000, None])
+@pytest.mark.parametrize("scores", [False, True])
+def test_attention_with_any_bound_on_the_lengths(rib, lib, max_len, scores):
+    """max_len chooses how units are split, and with it the order of the sums; every choice is within the bounds."""
+    check_attention(rib, lib, [200, 3, 0, 77], nq=8, nkv=2, D=128, page_rows=16, dtype=BF16, max_len=max_len, width=80,
+                    scores=scores)
