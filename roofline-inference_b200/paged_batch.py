@@ -87,6 +87,10 @@ class PagedDecoder:
         if pool.storage.shape[0] != cfg.num_layers or pool.n_kv != engine.n_kv or pool.storage.shape[5] != HEAD_DIM \
                 or pool.storage.dtype != torch.bfloat16:
             raise ValueError("the pool does not match the engine's layers / KV heads")
+        if pool.storage.device != dev:
+            raise ValueError(f"the pool is on {pool.storage.device}, the engine on {dev}")
+        if rotary is not None and (rotary.head_dim != HEAD_DIM or rotary.device != dev):
+            raise ValueError(f"rotary must rotate heads of {HEAD_DIM} dims on {dev}")
         if slots < 1 or max_rows < 1:
             raise ValueError("need at least one slot and max_rows >= 1")
         if keep is not None and (not 1 <= keep < max_rows or sinks < 0 or recent < 0 or sinks + recent > keep):

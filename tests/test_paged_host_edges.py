@@ -182,3 +182,16 @@ def test_yarn_stretches_every_pair_of_a_short_original_length(rib, length, slow)
     g, _ = paged.rotary_frequencies(64, 1e4, "yarn", 4.0, length, slow_turns=slow)
     assert length < 2 * math.pi * slow
     assert g == [x / 4 for x in f]
+
+
+@pytest.mark.parametrize("what", ["pool", "rotary device", "rotary dims"])
+def test_decoder_refuses_what_its_calls_could_not_use(rib, what):
+    """A pool or a rotation on another device, or a rotation of other heads, is refused when the decoder is made."""
+    d, pool = decoder(rib, [3], pages=6, max_rows=64)
+    rotary = None
+    if what == "pool":
+        pool = rib.PagePool(2, 1, 6, 16, device="meta")
+    else:
+        rotary = rib.Rotary(128, device="meta") if what == "rotary device" else rib.Rotary(64, device="cpu")
+    with pytest.raises(ValueError):
+        rib.PagedDecoder(d.e, pool, 1, 64, rotary=rotary)
