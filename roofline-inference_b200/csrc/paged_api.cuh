@@ -49,7 +49,7 @@ int rotary_ok(const rib_rotary *r, int dim) {
   return (reinterpret_cast<uintptr_t>(r->turns) & 7u) ? RIB_EALIGN : RIB_OK;
 }
 
-bool g_append_smem_done[2][5][kMaxDevices];
+bool g_append_smem_done[2][4][kMaxDevices];
 
 template <class T, int LANES>
 int append_launch_lanes(rib::paged::AppendParams &p, cudaStream_t st) {
