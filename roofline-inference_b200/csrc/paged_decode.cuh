@@ -17,17 +17,20 @@
 // a ring of ST slots of the warp's own by TMA (one 5-D box per 64 dims: 16 rows of K and of V of one
 // page), so warps never wait for each other within a unit.  Scores and P.V run on mma.m16n8k16 with
 // the heads as the 16 rows.  A decode step reads 4 D bytes per row for 4 D flops per query head, so
-// memory bounds it at any group size here (8 heads per KV head: 52 TFLOP/s at the full memory rate), and
+// memory bounds it up to 16 heads per KV head (8 heads: 52 TFLOP/s at the full memory rate), and
 // a tcgen05 tile (128 rows at least, accumulators in TMEM) would add a round trip through TMEM for rows
-// that stay empty.  With 8 heads the upper 8 rows of the A operand are free: in P.V they carry
-// p - round(p), so P enters with 16 (BF16) or 22 (FP16) bits and its rounding adds nothing to the
-// output's.  FP16 weights are lifted by 2^14 (as is their sum), out of the type's subnormal range: many
-// small weights behind one large one add up.  With more than 8 heads per KV head all 16 rows are heads, so
-// the rows are still read once, and the rounding's part is a second mma.
+// that stay empty.  Beyond 16 heads the rows are read once for every 16 (64 x 8-9k rows: 16 heads over one
+// 53 us, 32 over one 93).  With 8 heads the upper 8 rows of the A operand are free: in P.V they carry
+// p - round(p), so P enters with 16 (BF16) or 22 (FP16) bits.  That rounding is 2^-9 of the output's own; a
+// third part of P took 3 to 8 % longer in short calls and with 16 heads, and spilled registers.  FP16 weights
+// are lifted by 2^14 (as is their sum; in the exponent, which costs them 2^-21), out of the type's subnormal
+// range: many small weights behind one large one add up.  With more than 8 heads per KV head all 16 rows are
+// heads, so the rows are still read once, and the rounding's part is a second mma.  Scores, maxima, sums of
+// weights and sums over P.V are FP32.
 //
 // Measured on B200 (one launch pair, state larger than L2): 64 sequences of 30-33k rows, 8 KV heads of
-// 64 dims, 605-633 us (6.5-6.8 TB/s); 32 x 8191 rows, 64 heads over 8, FP16, 165-169 us (6.4-6.5 TB/s,
-// DRAM reads 1.000 of the rows' bytes); 64 x 512-4096 rows with row weights 108-110 us (of them 13 us for
+// 64 dims, 600-640 us (6.4-6.9 TB/s); 32 x 8191 rows, 64 heads over 8, FP16, 165-169 us (6.4-6.5 TB/s,
+// DRAM reads 1.000 of the rows' bytes); 64 x 512-4096 rows with row weights 108-111 us (of them 13-16 us for
 // join and weights); 1 x 32769 rows 30 us, of which the copies take 20.
 #pragma once
 

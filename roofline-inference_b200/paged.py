@@ -8,7 +8,8 @@ query heads per KV head are the caller's.
 
   pages  [num_pages, 2, nkv, page_rows, head_dim] BF16 or FP16 (K, then V); any strides that are
          multiples of 8 values with the last dimension contiguous, e.g. one layer of a pool
-         [num_pages, layers, 2, nkv, page_rows, head_dim]
+         [num_pages, layers, 2, nkv, page_rows, head_dim], in any order in memory.  head_dim is a
+         multiple of 16 from 32 to 256 for the append, 64 or 128 for attention and eviction
   table  [sequences, width] int32: the pages of each sequence in order (row r in page
          table[s, r // page_rows]); entries behind a sequence's rows are never read
 
@@ -128,13 +129,17 @@ def paged_decode_attention(q, pages, table, lens, scale: float, *, max_len: int 
     """Attention of one new token per sequence over its lens[b] rows; returns [B, nq, D].
 
     q [B, nq, D]; nq any multiple of nkv; D 64 or 128; page_rows a multiple of 16; lens int32 CUDA [B]
-    (0: the output row is zeros).  max_len: host bound on lens (what the table holds by default); it
-    sizes nothing but the scores' scratch.  scores [B, nkv, >= max_len] FP32: the softmax weight of
+    (0: the output row is zeros, as where every score is -infinity).  max_len: host bound on lens (what
+    the table holds by default); a longer length is cut to it and reported.  It sizes the launch and, with
+    scores, the scratch (4 B * nq * max_len bytes), and with it at most 256 rows are attended in one launch
+    instead of two: worth giving for short sequences in a wide table.  The order of the sums, and so the
+    last bits, may differ with it.  scores [B, nkv, >= max_len] FP32: the softmax weight of
     each row, summed over the query heads of its KV head, is added to it, in place or into scores_out
     (scores itself, or a buffer that does not overlap it); entries behind lens[b] stay as they are.
     Infinite V values give infinities, NaN where both signs meet, NaN gives NaN: every row's weight counts
     as positive, however small.
-    Weights and sums are FP32; the result is rounded once."""
+    Scores, weights and all sums are FP32; a weight enters its product with V in two parts of the pages'
+    type (16 bits for BF16, 22 for FP16), and the result is rounded once."""
     return _lib.binding().paged_decode_attention(q, pages, table, lens, scale, max_len, scores, scores_out, out)
 
 

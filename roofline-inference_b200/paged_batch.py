@@ -76,8 +76,9 @@ class PagedDecoder:
 
     rotary: the rotation (default: the engine's base, whole head).  keep: with it, a sequence that has
     filled max_rows is cut to its `keep` best rows before the next step (its first `sinks`, its last
-    `recent` and those that decode steps gave the most attention, per layer and KV head); without it
-    such a sequence raises "KV capacity exceeded"."""
+    `recent` and those that decode steps gave the most attention, per layer and KV head; a prompt's rows
+    start with none, so one that fills max_rows is cut, before its first step, to its lowest rows between
+    those); without it such a sequence raises "KV capacity exceeded"."""
 
     def __init__(self, engine, pool: PagePool, slots: int, max_rows: int, *, rotary: Rotary | None = None,
                  keep: int | None = None, sinks: int = 4, recent: int = 32):
