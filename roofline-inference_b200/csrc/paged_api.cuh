@@ -187,7 +187,7 @@ int paged_decode_launch(const rib::paged::DecodeParams &p, int dim, int grid, cu
 }
 
 // Units of 8 query heads, or of 16 where a KV head has more than 8: its rows are read once per unit (64 x
-// 8-9k rows, 16 heads over one of 128 dims: 52 us, as two units of 8 88; with 8 heads, 16 would do twice
+// 8-9k rows, 16 heads over one of 128 dims: 53 us, as two units of 8 88; with 8 heads, 16 would do twice
 // the P.V products for nothing).
 inline int unit_heads(int group) { return group <= 8 ? 8 : 16; }
 
