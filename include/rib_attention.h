@@ -707,7 +707,8 @@ int rib_paged_append(const rib_paged_cache *cache, const rib_rotary *rot,
  * lens[b] == 0 gives a row of zeros.  What pages hold behind a sequence's rows
  * (infinities, NaN) has no effect.  Infinite V values within them give
  * infinities, NaN where both signs meet, NaN gives NaN: every row's weight
- * counts as positive, however small.
+ * counts as positive, however small.  Where every score is -infinity the
+ * output is zeros.
  * With `scores` and `scores_out` (FP32
  * [batch][nkv][>= max_len], rows contiguous; they may be the same buffer):
  *   scores_out[b][h][n] = scores[b][h][n] + the softmax weight of row n

@@ -96,6 +96,39 @@ def test_attention_infinite_and_nan_values(rib, lib, low, n, nq, nkv, D, dtype):
     assert ((a - w).abs() <= w.abs() * half_step(dtype) + smallest_half(dtype) + b).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("nq,nkv,D", [(4, 2, 64), (16, 1, 128)])
+@pytest.mark.parametrize("n", [1, 250, 6000])
+def test_attention_scores_of_minus_infinity(rib, lib, n, nq, nkv, D, dtype):
+    """Rows whose keys make their scores -infinity get no weight; where all do, the output is zeros and no row's
+    score changes."""
+    g = gen(n)
+    pages, table = make_cache([n, n], nkv, D, 16, dtype, g)
+    clean = pages.clone()
+    at = torch.arange(n, device="cuda")
+    pages[table[0, at // 16].long(), 0, :, at % 16, 0] = -math.inf        # sequence 0: every row
+    some = at[(at % 3 > 0) | (at < n // 2)] if n > 1 else at[:0]            # sequence 1: most rows
+    pages[table[1, some // 16].long(), 0, :, some % 16, 0] = -math.inf
+    q = torch.randn((2, nq, D), generator=g).to(dtype).cuda()
+    q[..., 0] = 1.0
+    old = torch.rand((2, nkv, table.shape[1] * 16), generator=g).cuda()
+    scores = old.clone()
+    got = rib.paged_decode_attention(q, pages, table, i32([n, n]), D ** -0.5, scores=scores)
+    assert lib.take_device_status() == 0
+    assert (got[0] == 0).all() and torch.equal(scores[0], old[0])
+    # sequence 1: attention over the rows that are left, gathered into pages of their own
+    left = at[~torch.isin(at, some)]
+    m = left.numel()
+    short, one = make_cache([m], nkv, D, 16, dtype, g)
+    to = torch.arange(m, device="cuda")
+    short[one[0, to // 16].long(), :, :, to % 16] = clean[table[1, left // 16].long(), :, :, left % 16]
+    want, weights, bound, rel = attend64(q[1:], short, one, [m], D ** -0.5)
+    assert ((got[1:].double() - want).abs() <= want.abs() * half_step(dtype) + smallest_half(dtype) + bound).all()
+    expect = old[1, :, left].double() + weights[0]
+    assert ((scores[1, :, left].double() - expect).abs() <= expect * 2.0 ** -24 + weights[0] * rel[0]).all()
+    assert torch.equal(scores[1, :, some], old[1, :, some]) and torch.equal(scores[1, :, n:], old[1, :, n:])
+
+
 # ------------------------------------------------------------------ eviction
 def test_evict_keep_is_bounded(rib, lib):
     """`keep` beyond what the loops over rows count to is refused on the host, before its buffers are made."""
